@@ -1,0 +1,629 @@
+"""The operators around a decoding step over a cache in 8 bits, as calls that can be timed and checked.
+
+A step of the engine takes the projections' rows, rotates Q and K to their positions, stores K and V, attends to the
+cache, and at its end decides which drafted tokens stay:
+
+  rope    rotary positions of Q and K: half and interleaved pairs, a part of the head or all of it, frequencies
+          scaled for long contexts, with or without the RMS norm in front of it; f32 or f16 rows
+  store   K and V rows quantised into the 8-bit cache as they are written (a scale for each 32 cells of a head, which
+          grows with the rows that arrive) and the cells read back as f16 rows
+  attend  attention over that cache: one token, a drafted block, a prompt chunk; one range of cells per stream or
+          shuffled 256-cell pages; lengths as the mask, or a mask handed over (a tree of drafts)
+  draft   drafted tokens against the target's probabilities, from given random numbers: the rows kept and the token
+          behind them
+
+`own` says which side runs: the plain form in elementary torch operations, or this framework's calls. Inputs are on the
+GPU before a pass; buffers and the calls' handles are kept from pass to pass.
+"""
+from __future__ import annotations
+
+import math
+import pathlib
+import sys
+
+import torch
+
+own = False
+
+H, HKV = 24, 4          # query heads and kv-heads of the engine's model
+BLOCK, PAGE = 32, 256   # cells that share a scale, cells of a page
+EPS = 1e-6
+E_MIN, E_MAX = -40, 40  # range of a block's scale exponent
+
+
+def _framework():
+    root = str(pathlib.Path(__file__).resolve().parents[1] / "sixi-asi_amd")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import sixi_attn
+
+    return sixi_attn
+
+
+# ---- cases ----
+
+def _rope(name, streams, rows, dim, rot, layout, start, scaled, norm, dtype):
+    return {"name": name, "kind": "rope", "streams": streams, "rows": rows, "dim": dim, "rot": rot, "layout": layout,
+            "start": start, "scaled": scaled, "norm": norm, "dtype": dtype}
+
+
+def _store(name, streams, rows, dim, lo, hi, paged, dtype, ragged=False):
+    return {"name": name, "kind": "store", "streams": streams, "rows": rows, "dim": dim, "cached_lo": lo,
+            "cached_hi": hi, "paged": paged, "dtype": dtype, "ragged": ragged}
+
+
+def _attend(name, streams, rows, lo, hi, dim, paged=False, tree=False, ragged=False):
+    return {"name": name, "kind": "attend", "streams": streams, "rows": rows, "cached_lo": lo, "cached_hi": hi,
+            "dim": dim, "paged": paged, "tree": tree, "ragged": ragged}
+
+
+def _draft(name, streams, rows, vocab, probs, dtype, greedy=False, ragged=False):
+    return {"name": name, "kind": "draft", "streams": streams, "rows": rows, "vocab": vocab, "probs": probs,
+            "dtype": dtype, "greedy": greedy, "ragged": ragged}
+
+
+def listed():
+    return [
+        # one user's next token in the engine's model: norm, a quarter of the head rotated; launch and latency
+        _rope("rope_token", 1, 1, 256, 64, "half", 9000, False, True, "f32"),
+        # a prompt chunk far into a long context: whole heads in interleaved pairs, scaled frequencies
+        _rope("rope_chunk_long", 1, 2048, 128, 128, "interleaved", 180000, True, False, "f16"),
+        # the next token of every slot of a full server
+        _store("store_tokens", 32, 1, 128, 512, 15873, True, "f32"),
+        # a prompt chunk into one user's cache, starting inside a block of cells
+        _store("store_chunk", 1, 2048, 256, 4111, 4111, False, "f16"),
+        # one user, one token at a time: the smallest attention call
+        _attend("decode_one", 1, 1, 4095, 4095, 256),
+        # a full server's decode step out of the page pool, contexts of 0.5k to 16k
+        _attend("decode_batch", 32, 1, 512, 15873, 128, paged=True),
+        # the same server verifying 16-token drafts
+        _attend("verify_batch", 32, 16, 512, 15873, 128, paged=True),
+        # a few users' draft trees of 12 tokens, the tree as a mask
+        _attend("verify_tree", 8, 12, 2000, 9001, 256, tree=True),
+        # a prompt's middle chunk
+        _attend("prefill_chunk", 1, 2048, 4096, 4096, 128),
+        # the next turn of a chat: a short prompt behind a long cached context
+        _attend("chat_turn", 1, 173, 11400, 11400, 256, paged=True),
+        # one user's short draft, the drafter's own distribution known
+        _draft("draft_one", 1, 5, 131072, True, "f32"),
+        # a full server's verify step: sampled and greedy requests, drafts of different lengths
+        _draft("draft_batch", 32, 16, 131072, True, "f32", ragged=True),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+MAX_BYTES, MAX_FLOPS = 2.6e8, 1.25e11  # within the largest listed cases
+
+
+def draw(rng):
+    kind = rng.choice(("rope", "store", "attend", "attend", "attend", "draft"))
+    dim = rng.choice((128, 256))
+    if kind == "rope":
+        streams = _log_int(rng, 1, 32)
+        case = _rope("", streams, rng.randint(1, 16) if streams > 2 else _log_int(rng, 1, 2048), dim,
+                     dim if rng.random() < 0.5 else dim // 4, rng.choice(("half", "interleaved")),
+                     _log_int(rng, 1, 200000), rng.random() < 0.5, rng.random() < 0.5, rng.choice(("f32", "f16")))
+    elif kind == "store":
+        streams = _log_int(rng, 1, 32)
+        hi = _log_int(rng, 1, 16000)
+        case = _store("", streams, rng.randint(1, 16) if streams > 2 else _log_int(rng, 1, 2048), dim,
+                      rng.randint(0, hi), hi, rng.random() < 0.5, rng.choice(("f32", "f16")),
+                      streams > 1 and rng.random() < 0.5)
+    elif kind == "attend":
+        if rng.random() < 0.6:
+            streams, rows = _log_int(rng, 1, 32), rng.randint(1, 16)
+            hi = _log_int(rng, 100, 16384 if streams > 8 else 60000)
+        else:
+            streams, rows = rng.choice((1, 1, 1, 2, 4)), _log_int(rng, 17, 2048)
+            hi = _log_int(rng, 64, 30000)
+        lo = max(1, int(hi * rng.uniform(0.1, 1.0))) if streams > 1 else hi
+        paged = rng.random() < 0.5
+        case = _attend("", streams, rows, lo, hi, dim, paged, 2 < rows <= 16 and rng.random() < 0.4,
+                       streams > 1 and rng.random() < 0.5)
+    else:
+        streams = _log_int(rng, 1, 32)
+        case = _draft("", streams, rng.randint(1, 16), _log_int(rng, 1000, 140000), rng.random() < 0.6,
+                      rng.choice(("f32", "f16")), rng.random() < 0.25, streams > 1 and rng.random() < 0.5)
+    del case["name"]
+    while work(case)["bytes"] > MAX_BYTES or work(case)["flops"] > MAX_FLOPS:
+        for key, least in (("vocab", 1000), ("cached_hi", 64)):
+            if case.get(key, 0) > least:
+                case[key] = max(least, int(case[key] * 0.8))
+        if "cached_lo" in case:
+            case["cached_lo"] = min(case["cached_lo"], case["cached_hi"])
+        if case["rows"] > 16 and case.get("cached_hi", 0) <= 4096:
+            case["rows"] = max(17, int(case["rows"] * 0.9))
+    return case
+
+
+# ---- sizes ----
+
+def _spread(n, lo, hi):
+    """n values over [lo, hi], both ends among them, in no order (a fixed shuffle by a step coprime to n)."""
+    if n == 1:
+        return [hi]
+    step = next(k for k in range(n // 2 + 1, 2 * n) if math.gcd(k, n) == 1)
+    return [lo + (hi - lo) * (i * step % n) // (n - 1) for i in range(n)]
+
+
+def _lengths(case):
+    """(cached cells, rows) of each stream."""
+    cached = _spread(case["streams"], case.get("cached_lo", 0), case.get("cached_hi", 0))
+    rows = [case["rows"]] * case["streams"]
+    if case.get("ragged"):
+        rows = _spread(case["streams"], (case["rows"] + 1) // 2, case["rows"])[::-1]
+    return cached, rows
+
+
+def work(case):
+    cached, rows = _lengths(case)
+    n, es = sum(rows), 2 if case.get("dtype") == "f16" else 4
+    if case["kind"] == "rope":
+        return {"bytes": 2 * n * (H + HKV) * case["dim"] * es, "flops": 6 * n * (H + HKV) * case["dim"]}
+    if case["kind"] == "store":
+        # rows in, codes out; the kept cells of a block that is begun are read and may change; cells read back as f16
+        kept = sum(c % BLOCK for c in cached)
+        return {"bytes": 2 * HKV * case["dim"] * (n * (es + 1) + 2 * kept + (n + kept) * 3), "flops": 0}
+    if case["kind"] == "attend":
+        d = case["dim"]
+        seen = sum(r * c + (r * (r + 1) // 2) for c, r in zip(cached, rows))
+        moved = 2 * HKV * d * sum(c + r for c, r in zip(cached, rows)) + 2 * n * H * d * 2
+        if case["tree"]:
+            moved += 2 * sum(r * (c + r) for c, r in zip(cached, rows))
+        return {"bytes": moved, "flops": 4 * d * H * seen}
+    # every row's logits once; of the drafter's distributions the drafted tokens' entries and one row of each stream
+    return {"bytes": n * case["vocab"] * es + (case["streams"] * case["vocab"] * 4 if case["probs"] else 0),
+            "flops": 4 * n * case["vocab"]}
+
+
+# ---- inputs ----
+
+_TYPES = {"f32": torch.float32, "f16": torch.float16}
+
+
+def _i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def _frequencies(rot, scaled):
+    """Radians per position of each pair (64 bits) and the factor on the rotated rows: base 1e7; scaled by 8 from
+    a trained context of 32768 positions, the slow pairs stretched and the fast ones left (YaRN)."""
+    base, i = 1e7, torch.arange(rot // 2, dtype=torch.float64)
+    f = base ** (-2.0 * i / rot)
+    if not scaled:
+        return f.cuda(), 1.0
+    factor, trained, fast, slow = 8.0, 32768, 32.0, 1.0
+    at = [rot * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base)) for turns in (fast, slow)]
+    lo, hi = max(0, math.floor(at[0])), min(rot - 1, math.ceil(at[1]))
+    stretch = ((i - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+    return (f / factor * stretch + f * (1 - stretch)).cuda(), 0.1 * math.log(factor) + 1.0
+
+
+def _cache(gen, case, cached, rows):
+    """K and V codes with their exponents, and the page table. K of a block of 32 cells lies as [dim / 16, cell, 16],
+    V as [dim, cell]; [streams, kv-heads, blocks, ...], or pages in the place of streams, at shuffled places."""
+    pages = [-(-(c + r) // PAGE) for c, r in zip(cached, rows)]
+    n, blocks = (sum(pages), PAGE // BLOCK) if case["paged"] else (case["streams"], max(pages) * PAGE // BLOCK)
+    d = case["dim"]
+
+    def codes(*shape):
+        # scales are set by the largest of the block's values, so most codes are small
+        x = torch.randn(shape, generator=gen, device="cuda", dtype=torch.float16)
+        return x.mul_(24).round_().clamp_(-127, 127).to(torch.int8)
+
+    def exponents():
+        return torch.randint(-6, -3, (n, HKV, blocks), generator=gen, device="cuda", dtype=torch.int8)
+
+    cache = {"k": codes(n, HKV, blocks, d // 16, BLOCK, 16), "k_exp": exponents(),
+             "v": codes(n, HKV, blocks, d, BLOCK), "v_exp": exponents()}
+    table = None
+    if case["paged"]:
+        order = torch.randperm(n, generator=gen, device="cuda").to(torch.int32)
+        table = torch.zeros((case["streams"], max(pages)), dtype=torch.int32, device="cuda")
+        at = 0
+        for i, p in enumerate(pages):
+            table[i, :p] = order[at:at + p]
+            at += p
+    return cache, table
+
+
+def _tree_mask(gen, cached, rows, n_rows, n_cells):
+    """f16 mask of drafted trees: every row sees the cached cells, itself and its ancestors (its parent is one of the
+    rows before it); a row behind its stream's last sees nothing. The hidden cells hold -inf or the type's lowest."""
+    s = len(cached)
+    seen = torch.eye(n_rows, dtype=torch.bool, device="cuda").repeat(s, 1, 1)
+    parent = (torch.rand((s, n_rows), generator=gen, device="cuda") * torch.arange(n_rows, device="cuda")).long()
+    for j in range(1, n_rows):
+        seen[:, j] |= seen[torch.arange(s, device="cuda"), parent[:, j]]
+    cell = torch.arange(n_cells, device="cuda")
+    at = cell - _i32(cached)[:, None]                                   # a cell's row of the block
+    inside = seen.gather(2, at.clamp(0, n_rows - 1)[:, None].expand(s, n_rows, n_cells))
+    shown = (at < 0)[:, None] | (inside & (at < n_rows)[:, None])
+    shown &= (torch.arange(n_rows, device="cuda") < _i32(rows)[:, None])[:, :, None]
+    hidden = torch.full((n_cells,), -math.inf, device="cuda")
+    hidden[::2] = torch.finfo(torch.float16).min
+    return torch.where(shown, 0.0, hidden).to(torch.float16)[:, None].contiguous()
+
+
+def _inputs(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    cached, rows = _lengths(case)
+    s, n, d = case["streams"], case["rows"], case.get("dim")
+    st = {"case": case, "q_len": _i32(rows)}
+
+    def randn(*shape):
+        return torch.randn(shape, generator=gen, device="cuda")
+
+    def rand(*shape):
+        return torch.rand(shape, generator=gen, device="cuda")
+
+    if case["kind"] == "rope":
+        t = _TYPES[case["dtype"]]
+        st.update(q=randn(s, n, H, d).to(t), k=randn(s, n, HKV, d).to(t),
+                  kv_len=_i32(_spread(s, case["start"] // 2, case["start"])))
+        st["freqs"], st["mscale"] = _frequencies(case["rot"], case["scaled"])
+        if case["norm"]:
+            st.update(q_norm=1 + 0.2 * randn(d), k_norm=1 + 0.2 * randn(d))
+        return st
+    if case["kind"] == "draft":
+        t, v = _TYPES[case["dtype"]], case["vocab"]
+        logits = 3.0 * randn(s, n, v)
+        # the drafter's view of the same rows; a sampler's filter has struck some tokens from the target
+        guess = torch.softmax(logits[:, :n - 1] + 0.7 * randn(s, n - 1, v), dim=-1)
+        logits.masked_fill_(rand(s, 1, v) < 0.1, -math.inf)
+        st.update(logits=logits.to(t), u=rand(s, n - 1), u_next=rand(s),
+                  draft=torch.zeros((s, 0), dtype=torch.int32, device="cuda"),
+                  temperature=0.6 + 0.6 * rand(s))
+        if n > 1:
+            pick = torch.multinomial(guess.reshape(-1, v), 1, generator=gen) if case["probs"] else guess.argmax(-1)
+            st["draft"] = pick.reshape(s, n - 1).to(torch.int32)
+        if case["greedy"]:
+            st["temperature"][::2] = 0.0
+        if case["probs"]:
+            st["draft_probs"] = guess
+        return st
+    st["cache"], st["table"] = _cache(gen, case, cached, rows)
+    st["kv_len"] = _i32(cached)
+    if case["kind"] == "store":
+        t = _TYPES[case["dtype"]]
+        # a stream's rows grow and shrink, so that some blocks' scales grow
+        size = torch.exp(1.5 * randn(s, n, HKV, 1) - 1.0)
+        st.update(k=(size * randn(s, n, HKV, d)).to(t), v=(size * randn(s, n, HKV, d)).to(t))
+        st["from"] = _i32([c // BLOCK * BLOCK for c in cached])
+        st["count"] = _i32([c % BLOCK + r for c, r in zip(cached, rows)])
+        return st
+    st["q"] = (2.0 * randn(s, n, H, d)).half()
+    if case["tree"]:
+        n_cells = st["table"].shape[1] * PAGE if case["paged"] else st["cache"]["k"].shape[2] * BLOCK
+        st["mask"] = _tree_mask(gen, cached, rows, n, n_cells)
+    return st
+
+
+def prepare(case, seed):
+    st = _inputs(case, seed)
+    s, n, d = case["streams"], case["rows"], case.get("dim")
+
+    def zeros(*shape, dtype):
+        return torch.zeros(shape, dtype=dtype, device="cuda")
+
+    if case["kind"] == "rope":
+        st["q_out"], st["k_out"] = torch.zeros_like(st["q"]), torch.zeros_like(st["k"])
+    elif case["kind"] == "store":
+        st["k_back"], st["v_back"] = (zeros(s, n + BLOCK - 1, HKV, d, dtype=torch.float16) for _ in range(2))
+    elif case["kind"] == "attend":
+        st["out"] = zeros(s, n, H, d, dtype=torch.float16)
+    else:
+        st["keep"], st["token"] = zeros(s, dtype=torch.int32), zeros(s, dtype=torch.int32)
+    return st
+
+
+# ---- one pass ----
+
+def run(st):
+    return _RUN[st["case"]["kind"]](st)
+
+
+def _run_rope(st):
+    if own:
+        sa = _framework()
+        case = st["case"]
+        sa.qk_rope(st["q"], st["k"], st["freqs"], st["q_out"], st["k_out"], kv_len=st["kv_len"], q_len=st["q_len"],
+                   layout=sa.ROPE_HALF if case["layout"] == "half" else sa.ROPE_INTERLEAVED, mscale=st["mscale"],
+                   q_norm=st.get("q_norm"), k_norm=st.get("k_norm"), eps=EPS)
+        return {"q": st["q_out"], "k": st["k_out"]}
+    return _plain_rope(st)
+
+
+def _run_store(st):
+    if own:
+        sa = _framework()
+        c = st["cache"]
+        if "kv8" not in st:
+            st["kv8"] = sa.Kv8Cache(c["k"], c["k_exp"], c["v"], c["v_exp"])
+        sa.kv8_write(st["k"], st["v"], st["kv8"], kv_len=st["kv_len"], q_len=st["q_len"], page_table=st["table"])
+        sa.kv8_read(st["kv8"], st["k_back"], st["v_back"], kv_len=st["from"], q_len=st["count"],
+                    page_table=st["table"])
+        return {"k": st["k_back"], "v": st["v_back"]}
+    return _plain_store(st)
+
+
+def _run_attend(st):
+    if own:
+        sa = _framework()
+        c = st["cache"]
+        if "kv8" not in st:
+            st["kv8"], st["handle"] = sa.Kv8Cache(c["k"], c["k_exp"], c["v"], c["v_exp"]), sa.Kv8Attention()
+        more = {"mask_mode": sa.MASK_EXPLICIT, "mask": st["mask"]} if "mask" in st else {}
+        st["handle"](st["q"], st["kv8"], st["out"], kv_len=st["kv_len"], q_len=st["q_len"], page_table=st["table"],
+                     **more)
+        return st["out"]
+    return _plain_attend(st)
+
+
+def _run_draft(st):
+    if own:
+        sa = _framework()
+        if "handle" not in st:
+            st["handle"] = sa.DraftVerify()
+        st["handle"](st["logits"], st["draft"], st["u"], st["u_next"], st["keep"], st["token"],
+                     draft_probs=st.get("draft_probs"), q_len=st["q_len"], temperature=st["temperature"])
+        return {"keep": st["keep"], "token": st["token"]}
+    return _plain_draft(st)
+
+
+_RUN = {"rope": _run_rope, "store": _run_store, "attend": _run_attend, "draft": _run_draft}
+
+
+# ---- plain forms ----
+
+def _plain_rope(st):
+    case = st["case"]
+    rows = torch.arange(case["rows"], device="cuda")
+    angle = (st["kv_len"][:, None] + rows).double()[:, :, None, None] * st["freqs"]  # 64 bits: far positions
+    cos, sin = ((f(angle) * st["mscale"]).float() for f in (torch.cos, torch.sin))
+    live = (rows < st["q_len"][:, None])[:, :, None, None]
+
+    def turn(x, weight, out):
+        x = x.float()
+        if weight is not None:
+            x = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + EPS) * weight
+        r = case["rot"]
+        if case["layout"] == "half":
+            a, b = x[..., :r // 2], x[..., r // 2:r]
+            y = torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1)
+        else:
+            a, b = x[..., 0:r:2], x[..., 1:r:2]
+            y = torch.stack([a * cos - b * sin, b * cos + a * sin], dim=-1).flatten(-2)
+        y = torch.cat([y, x[..., r:]], dim=-1).to(out.dtype)
+        return torch.where(live, y, out)
+
+    return {"q": turn(st["q"], st.get("q_norm"), st["q_out"]), "k": turn(st["k"], st.get("k_norm"), st["k_out"])}
+
+
+def _values(codes, exponents, is_key):
+    """Cells of a cache as f32 rows: [streams or pages, cells, kv-heads, dim]."""
+    x = codes.permute(0, 2, 4, 1, 3, 5) if is_key else codes.permute(0, 2, 4, 1, 3)
+    x = x.flatten(4).float() if is_key else x.float()
+    return torch.ldexp(x, exponents.permute(0, 2, 1)[:, :, None, :, None].int()).flatten(1, 2)
+
+
+def _plain_store(st):
+    case, c = st["case"], st["cache"]
+    n, s = case["rows"], case["streams"]
+    first, count = st["kv_len"].long(), st["q_len"].long()
+    blocks = (n + 2 * BLOCK - 2) // BLOCK                        # blocks that a stream's rows may reach
+    block = first[:, None] // BLOCK + torch.arange(blocks, device="cuda")
+    cell = block[:, :, None] * BLOCK + torch.arange(BLOCK, device="cuda")
+    row = cell - first[:, None, None]
+    new = (row >= 0) & (row < count[:, None, None])              # [streams, blocks, 32]
+    touched = new.any(-1)
+    kept = touched & (block * BLOCK < first[:, None])
+    # where each block lies; blocks behind the last row are read at the last one's place and not written
+    block = torch.minimum(block, (first + count - 1).clamp_min(0)[:, None] // BLOCK)
+    if st["table"] is not None:
+        at, block = st["table"].long().gather(1, block * BLOCK // PAGE), block % (PAGE // BLOCK)
+    else:
+        at = torch.arange(s, device="cuda")[:, None].expand_as(block)
+    out = {}
+    for name in ("k", "v"):
+        codes, exps = c[name], c[name + "_exp"]
+        x = st[name].float()
+        x = x.gather(1, row.clamp(0, n - 1).reshape(s, -1, 1, 1).expand(-1, -1, *x.shape[2:]))
+        x = x.reshape(s, blocks, BLOCK, HKV, -1)
+        here = new[:, :, :, None, None]
+        top = torch.where(here & x.isfinite(), x.abs(), 0.0).amax((2, 4))
+        m, e = torch.frexp(top)
+        e = torch.where(top > 0, e - torch.where(m <= 127 / 128, 7, 6), E_MIN).clamp(E_MIN, E_MAX)
+        was = exps[at, :, block].int()
+        e = torch.where(kept[:, :, None], torch.maximum(e, was), e)[:, :, None, :, None]
+        old = codes[at, :, block]                                # [streams, blocks, kv-heads, ...]
+        old = old.permute(0, 1, 4, 2, 3, 5).flatten(4) if name == "k" else old.permute(0, 1, 4, 2, 3)
+        old = old.float()
+        again = torch.round(torch.ldexp(old, was[:, :, None, :, None] - e))
+        fresh = torch.round(torch.ldexp(x, -e)).clamp(-127, 127).nan_to_num(0.0)
+        code = torch.where(here, fresh, torch.where((cell < first[:, None, None])[:, :, :, None, None], again, old))
+        back = torch.ldexp(code, e).half().reshape(s, blocks * BLOCK, HKV, -1)[:, :n + BLOCK - 1]
+        told = torch.arange(back.shape[1], device="cuda") < st["count"][:, None]
+        keep = st[name + "_back"][:, :back.shape[1]]
+        out[name] = torch.cat([torch.where(told[:, :, None, None], back, keep), st[name + "_back"][:, back.shape[1]:]], 1)
+        code = code.to(torch.int8)
+        if name == "k":
+            code = code.reshape(s, blocks, BLOCK, HKV, -1, 16).permute(0, 1, 3, 4, 2, 5)
+        else:
+            code = code.permute(0, 1, 3, 4, 2)
+        codes[at[touched], :, block[touched]] = code[touched]
+        exps[at[touched], :, block[touched]] = e[:, :, 0, :, 0][touched].to(torch.int8)
+    return out
+
+
+def _plain_attend(st):
+    case, c, table = st["case"], st["cache"], st["table"]
+    s, n, d = case["streams"], case["rows"], case["dim"]
+    k, v = _values(c["k"], c["k_exp"], True), _values(c["v"], c["v_exp"], False)
+    if table is not None:
+        k, v = (x[table.long()].flatten(1, 2) for x in (k, v))
+    q = st["q"].float().reshape(s, n, HKV, H // HKV, d).permute(0, 2, 1, 3, 4).reshape(s, HKV, -1, d).contiguous()
+    score = torch.matmul(q, k.permute(0, 2, 3, 1).contiguous()) / d ** 0.5
+    score = score.reshape(s, HKV, n, H // HKV, -1)
+    cell, row = torch.arange(k.shape[1], device="cuda"), torch.arange(n, device="cuda")
+    if "mask" in st:
+        score += st["mask"].float()[:, :, :, None]
+        score.masked_fill_((cell >= (st["kv_len"] + st["q_len"])[:, None])[:, None, None, None], -math.inf)
+    else:
+        last = st["kv_len"][:, None] + row
+        score.masked_fill_((cell > last[:, :, None])[:, None, :, None], -math.inf)
+    top = score.amax(-1, keepdim=True)
+    score = torch.exp_(score.sub_(torch.where(top == -math.inf, 0.0, top)))
+    total = score.sum(-1, keepdim=True)
+    score = score.reshape(s, HKV, n * (H // HKV), -1)
+    out = torch.matmul(score, v.permute(0, 2, 1, 3).contiguous()).reshape(s, HKV, n, H // HKV, d)
+    out = torch.where(total > 0, out / total, 0.0).permute(0, 2, 1, 3, 4).reshape(s, n, H, d).half()
+    return torch.where((row < st["q_len"][:, None])[:, :, None, None], out, st["out"])
+
+
+def _plain_draft(st):
+    # 64 bits: a token is found where a long running sum passes a number, and many tokens lie close together there
+    logits, q = st["logits"].double(), st.get("draft_probs")
+    s, n, v = logits.shape
+    heat = st["temperature"].double()[:, None, None]
+    best = logits.argmax(-1, keepdim=True)
+    logits = logits / torch.where(heat > 0, heat, 1.0)
+    p = torch.exp(logits - logits.amax(-1, keepdim=True))
+    p = p / p.sum(-1, keepdim=True)
+    p = torch.where(heat > 0, p, torch.zeros_like(p).scatter_(-1, best, 1.0))
+    d = st["draft"].long()[:, :, None]
+    each = torch.arange(n, device="cuda")
+    ok = (each[:n - 1] < st["q_len"][:, None] - 1)
+    if n > 1:
+        asked = q.gather(-1, d)[:, :, 0].double() if q is not None else 1.0
+        ok = ok & (st["u"].double() * asked < p[:, :n - 1].gather(-1, d)[:, :, 0])
+    kept = ok.int().cumprod(-1).sum(-1)
+    p = p.gather(1, kept[:, None, None].expand(s, 1, v))[:, 0]
+    w = p
+    if n > 1:
+        at = kept.clamp_max(n - 2)[:, None, None]
+        if q is not None:
+            q = q.gather(1, at.expand(s, 1, v))[:, 0].double()
+        else:
+            q = torch.zeros_like(p).scatter_(-1, d.gather(1, at)[:, 0], 1.0)
+        w = torch.where((kept < st["q_len"] - 1)[:, None], (p - q).clamp_min(0), p)
+    w = torch.where(w.sum(-1, keepdim=True) > 0, w, p)
+    mark = st["u_next"].double()[:, None] * w.sum(-1, keepdim=True)
+    token = (w.cumsum(-1) <= mark).sum(-1)
+    last = torch.where(w > 0, torch.arange(v, device="cuda"), -1).amax(-1)
+    return {"keep": (kept + 1).to(torch.int32), "token": torch.minimum(token, last).to(torch.int32)}
+
+
+# ---- the same in 64 bits ----
+
+def exact(case, seed):
+    st = prepare(case, seed)
+    cached, rows = _lengths(case)
+    return {"rope": _exact_rope, "store": _exact_store, "attend": _exact_attend, "draft": _exact_draft}[case["kind"]](
+        st, case, cached, rows)
+
+
+def _exact_rope(st, case, cached, rows):
+    r, got = case["rot"], {}
+    for name in ("q", "k"):
+        x, y = st[name].double(), torch.zeros_like(st[name], dtype=torch.float64)
+        if case["norm"]:
+            x = x / torch.sqrt((x * x).sum(-1, keepdim=True) / x.shape[-1] + EPS) * st[name + "_norm"].double()
+        first, step = (slice(0, r // 2), slice(r // 2, r)) if case["layout"] == "half" else (slice(0, r, 2), slice(1, r, 2))
+        for i, n in enumerate(rows):
+            place = torch.arange(n, device="cuda", dtype=torch.float64) + float(st["kv_len"][i])
+            turn = st["mscale"] * torch.polar(torch.ones((), dtype=torch.float64, device="cuda"), place[:, None] * st["freqs"])
+            z = torch.complex(x[i, :n, :, first].contiguous(), x[i, :n, :, step].contiguous()) * turn[:, None]
+            y[i, :n] = x[i, :n]
+            y[i, :n, :, first], y[i, :n, :, step] = z.real, z.imag
+        got[name] = y
+    return got
+
+
+def _rows_of(cache, table, i, n, name):
+    """Cells 0 .. n-1 of stream i in 64 bits: codes [cells, kv-heads, dim] and exponents [blocks, kv-heads]."""
+    x, e = cache[name], cache[name + "_exp"]
+    if table is None:
+        x, e = x[i].transpose(0, 1), e[i].t()
+    else:
+        pages = table[i, :-(-n // PAGE)].long()
+        x, e = x[pages].transpose(1, 2).flatten(0, 1), e[pages].transpose(1, 2).flatten(0, 1)
+    x = x[:-(-n // BLOCK)].double()                              # [blocks, kv-heads, dim/16, 32, 16] or [.., dim, 32]
+    x = x.permute(0, 3, 1, 2, 4).flatten(3) if name == "k" else x.permute(0, 3, 1, 2)
+    return x, e[:-(-n // BLOCK)].double()
+
+
+def _exact_store(st, case, cached, rows):
+    got = {}
+    for name in ("k", "v"):
+        back = st[name + "_back"].double()
+        for i, (c, r) in enumerate(zip(cached, rows)):
+            x, e = _rows_of(st["cache"], st["table"], i, c + r, name)
+            x, e, new = x[c // BLOCK:], e[c // BLOCK:], st[name][i, :r].double()
+            blocks, kept = x.shape[0], c % BLOCK
+            rest = blocks * BLOCK - kept - r
+            padded = torch.nn.functional.pad(new, (0, 0, 0, 0, kept, rest)).reshape(blocks, BLOCK, HKV, -1)
+            top = padded.abs().amax((1, 3))
+            want = torch.ceil(torch.log2(top / 127)).clamp(E_MIN, E_MAX)
+            if kept:
+                want[0] = torch.maximum(want[0], e[0])
+            code = torch.round(padded * torch.exp2(-want)[:, None, :, None])
+            code = code.clamp(-127, 127)
+            if kept:
+                code[0, :kept] = torch.round(x[0, :kept] * torch.exp2(e[0] - want[0])[None, :, None])
+            value = (code * torch.exp2(want)[:, None, :, None]).flatten(0, 1)[:kept + r]
+            back[i, :kept + r] = value
+        got[name] = back
+    return got
+
+
+def _exact_attend(st, case, cached, rows):
+    d = case["dim"]
+    out = torch.zeros(st["out"].shape, dtype=torch.float64, device="cuda")
+    for i, (c, r) in enumerate(zip(cached, rows)):
+        k, v = ((x * torch.exp2(e)[:, None, :, None]).flatten(0, 1)[:c + r]
+                for x, e in (_rows_of(st["cache"], st["table"], i, c + r, name) for name in ("k", "v")))
+        if "mask" in st:
+            add = st["mask"][i, 0, :r, :c + r].double()
+        else:
+            hidden = torch.arange(c + r, device="cuda") > c + torch.arange(r, device="cuda")[:, None]
+            add = torch.zeros(hidden.shape, dtype=torch.float64, device="cuda").masked_fill_(hidden, -math.inf)
+        for h in range(H):
+            g = h // (H // HKV)
+            score = st["q"][i, :r, h].double() @ k[:, g].t().contiguous() * (1.0 / math.sqrt(d)) + add
+            out[i, :r, h] = torch.softmax(score, dim=-1) @ v[:, g].contiguous()
+    return out
+
+
+def _exact_draft(st, case, cached, rows):
+    keep, token = [], []
+    for i, r in enumerate(rows):
+        heat, j, w = float(st["temperature"][i]), 0, None
+        while w is None:
+            x = st["logits"][i, j].double()
+            if heat > 0:
+                p = torch.softmax(x / heat, dim=0)
+            else:
+                p = torch.zeros_like(x)
+                p[int(torch.nonzero(x == x.max())[0])] = 1.0
+            if j == r - 1:
+                w = p
+                break
+            q = st["draft_probs"][i, j].double() if case["probs"] else torch.zeros_like(p)
+            d = int(st["draft"][i, j])
+            if not case["probs"]:
+                q[d] = 1.0
+            if float(st["u"][i, j]) * float(q[d]) < float(p[d]):
+                j += 1
+                continue
+            w = torch.relu(p - q)
+            if not float(w.sum()) > 0:
+                w = p
+        run = torch.cumsum(w, 0)
+        past = torch.searchsorted(run, float(st["u_next"][i]) * run[-1], right=True)
+        keep.append(j + 1)
+        token.append(min(int(past), int(torch.nonzero(w)[-1])))
+    return {"keep": _i32(keep), "token": _i32(token)}
