@@ -2,7 +2,8 @@
 
     lib/libsixi_attn.so   gfx950 HIP kernels + the C ABIs of include/sixi_attn.h,
                           include/sixi_kv.h, include/sixi_plan.h,
-                          include/sixi_layer.h and include/sixi_gdn.h (hipcc)
+                          include/sixi_layer.h, include/sixi_gdn.h, include/sixi_kv8.h,
+                          include/sixi_rope.h and include/sixi_draft.h (hipcc)
     lib/libsixi_synth.so  seeded synthetic workload generator used by bench.py and tests (g++)
 
 Run as ``python sixi-asi_amd/build.py`` or through ``__graft_entry__.build()``.  Every call
@@ -52,7 +53,9 @@ def flags_for(src: str) -> list[str]:
 HIP_SOURCES = ["fa_decode.hip", "fa_prefill.hip", "fa_mask.hip", "fa_q8_stage.hip", "kv_write.hip", "sixi_attn_abi.cpp", "sixi_kv_abi.cpp",
                "sixi_kv_pool.cpp",
                "sixi_plan.cpp", "layer_prologue.hip", "sixi_layer_abi.cpp",
-               "gdn_verify.hip", "sixi_gdn_abi.cpp"]
+               "gdn_verify.hip", "sixi_gdn_abi.cpp",
+               "kv8_store.hip", "kv8_attn.hip", "sixi_kv8_abi.cpp", "rope.hip", "sixi_rope_abi.cpp",
+               "draft_verify.hip", "sixi_draft_abi.cpp"]
 
 
 def _hipcc() -> str:

@@ -6,6 +6,8 @@
 
 #include "sixi_attn.h"
 
+struct sixi_kv_pool;
+
 namespace sixi_abi {
 
 inline bool mul_ok(int64_t a, int64_t b, int64_t* out) { return !__builtin_mul_overflow(a, b, out); }
@@ -71,5 +73,12 @@ inline bool ranges_overlap(const void* a, int64_t a_bytes, const void* b, int64_
 inline bool views_overlap(const sixi_view& a, int64_t a_row, const sixi_view& b, int64_t b_row) {
     return ranges_overlap(a.data, view_span(a, a_row), b.data, view_span(b, b_row));
 }
+
+// A view whose rows are ne[0] bytes of any meaning (the page pool's copies).
+constexpr int32_t kRawBytes = -1;
+
+// Registers `n` views of raw bytes with the pool, all or none; ne[3] is the pool's page count.  The
+// caller has checked strides and spans.
+int pool_attach_raw(sixi_kv_pool* pool, const sixi_view* views, int n);
 
 }  // namespace sixi_abi

@@ -1,0 +1,48 @@
+// draft_internal.hpp -- kernel arguments shared by the draft verification's ABI (sixi_draft_abi.cpp) and
+// its kernels (draft_verify.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace sixi {
+
+constexpr int kDraftChunk = 4096;  // logits of a row that one work-group takes
+
+// A chunk of a row: the largest logit, the lowest token that has it, and the sum of exp((l - max) / T).
+struct DraftPart {
+    double sum;
+    float top;
+    int32_t at;
+};
+// A chunk of the row that the next token is drawn from: weights of the draw and of p, the last token with
+// a weight in each.
+struct DraftDraw {
+    double w, p;
+    int32_t last_w, last_p;
+};
+
+struct DraftArgs {
+    const char* logits;
+    int64_t l_nb1, l_nb2;  // row, stream
+    const char* probs;     // may be null
+    int64_t p_nb1, p_nb2;
+    int32_t l_type, p_type;
+    const int32_t* draft;
+    int64_t draft_stride;
+    const float* u;
+    int64_t u_stride;
+    const float* u_next;
+    const float* temperature;
+    const int32_t* q_len;
+    int32_t* keep;
+    int32_t* token;
+    DraftPart* parts;  // [S][n_rows][chunks]
+    DraftDraw* draws;  // [S][chunks]
+    int32_t V, n_rows, S, chunks;
+};
+
+hipError_t launch_draft_verify(const DraftArgs& a, hipStream_t stream);
+
+}  // namespace sixi

@@ -1,0 +1,75 @@
+// kv8_internal.hpp -- kernel arguments shared by the 8-bit cache's ABI (sixi_kv8_abi.cpp) and its
+// kernels (kv8_store.hip, kv8_attn.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sixi_kv8.h"
+
+namespace sixi {
+
+constexpr int kBlk = SIXI_KV8_BLOCK_CELLS;
+constexpr int kPageBlocks = SIXI_KV_PAGE_CELLS / SIXI_KV8_BLOCK_CELLS;
+
+// One tensor's codes and exponents (strides in bytes: block, head, stream or page).
+struct Kv8Tensor {
+    char* codes;
+    int8_t* exps;
+    int64_t nb[3];
+    int64_t e_nb[3];
+};
+
+// Where a stream's blocks lie.  pt null: block b of stream s at b * nb[0] + s * nb[2].
+struct Kv8Pages {
+    const int32_t* pt;
+    int64_t pt_stride;
+    int32_t n_pages;
+    int32_t n_blocks;  // blocks of a stream (paged: of its whole table row)
+};
+
+// Rows of both tensors against cells kv_len[s] + j.  Byte strides of the rows: row, head, stream.
+struct Kv8RowsArgs {
+    char* rows[2];
+    int64_t r_nb1[2], r_nb2[2], r_nb3[2];
+    int32_t f16[2];
+    Kv8Tensor t[2];
+    Kv8Pages pages;
+    const int32_t* kv_len;
+    const int32_t* q_len;
+    int32_t D, n_rows, Hkv, S;
+};
+
+hipError_t launch_kv8_write(const Kv8RowsArgs& a, hipStream_t stream);
+hipError_t launch_kv8_read(const Kv8RowsArgs& a, hipStream_t stream);
+
+struct Kv8AttnArgs {
+    const char* q;
+    int64_t q_nb1, q_nb2, q_nb3;  // row, head, stream
+    int32_t q_f16;
+    char* out;
+    int64_t o_nb1, o_nb2, o_nb3;  // head, row, stream
+    int32_t o_f16;
+    Kv8Tensor k, v;
+    Kv8Pages pages;
+    const int32_t* kv_len;
+    const int32_t* q_len;
+    const char* mask;             // EXPLICIT: f16 rows
+    int64_t m_nb1, m_nb3;         // row, stream (0: one for all)
+    int32_t mode;
+    int32_t S, H, Hkv, G, n_q, n_kv, D;
+    float scale_log2;             // |scale| * log2(e); the sign goes into Q
+    float q_sign;
+    float* part;                  // workspace
+    int32_t n_split, n_tiles;     // pieces of a stream's cells, 32-row tiles of a group's rows
+};
+
+hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t stream);
+
+// Pieces that a stream's cells are cut into.
+int kv8_attn_splits(int64_t S, int64_t Hkv, int64_t tiles, int64_t n_kv);
+// f32 values of the partial results of one (piece, tile).
+inline int64_t kv8_slot_floats(int D) { return 32 * (int64_t)D + 64; }
+
+}  // namespace sixi

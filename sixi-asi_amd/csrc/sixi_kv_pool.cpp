@@ -88,13 +88,13 @@ int copy_page(const sixi_kv_pool* p, int32_t from, int32_t to, hipStream_t strea
         a.nb1 = v.nb[1];
         a.nb2 = v.nb[2];
         a.nb3 = v.nb[3];
-        a.row_bytes = row_bytes(v.type, v.ne[0]);
+        a.row_bytes = v.type == kRawBytes ? v.ne[0] : row_bytes(v.type, v.ne[0]);
         a.Hkv = v.ne[2];
         a.src_stream = from;
         a.dst_stream = to;
         a.src_cell = 0;
         a.dst_cell = 0;
-        a.n_cells = kPage;
+        a.n_cells = v.ne[1];
         a.word4_aligned = aligned(v.data, 4) && v.nb[1] % 4 == 0 && v.nb[2] % 4 == 0 && v.nb[3] % 4 == 0;
         if (sixi::launch_kv_copy(a, stream) != hipSuccess) return SIXI_E_BACKEND;
     }
@@ -102,6 +102,20 @@ int copy_page(const sixi_kv_pool* p, int32_t from, int32_t to, hipStream_t strea
 }
 
 }  // namespace
+
+int sixi_abi::pool_attach_raw(sixi_kv_pool* pool, const sixi_view* views, int n) {
+    std::lock_guard<std::mutex> lock(pool->mu);
+    for (int i = 0; i < n; ++i)
+        if (views[i].ne[3] != pool->n_pages) return SIXI_E_INVALID_ARGUMENT;
+    if ((int)pool->views.size() + n > kMaxViews) return SIXI_E_OUT_OF_BOUNDS;
+    try {
+        pool->views.reserve(pool->views.size() + n);
+    } catch (const std::bad_alloc&) {
+        return SIXI_E_OUT_OF_BOUNDS;
+    }
+    pool->views.insert(pool->views.end(), views, views + n);
+    return SIXI_OK;
+}
 
 extern "C" {
 

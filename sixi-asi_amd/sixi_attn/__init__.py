@@ -27,6 +27,7 @@ LIB_PATH = LIB_DIR / "libsixi_attn.so"
 
 # ggml type ids
 TYPE_F32, TYPE_F16, TYPE_Q8_0 = 0, 1, 8
+TYPE_BF16 = 30  # draft_verify's logits and probabilities only
 # mask modes
 MASK_NONE, MASK_BLOCK_CAUSAL, MASK_EXPLICIT = 0, 1, 2
 # sixi_attn_params.flags; the f16 staging of a q8_0 cache stays under STAGE_CAP_BYTES
@@ -69,6 +70,19 @@ EXPORTED_SYMBOLS = (
     "sixi_qk_prologue",
     "sixi_attn_gate",
     "sixi_gdn_verify",
+    "sixi_kv8_write",
+    "sixi_kv8_read",
+    "sixi_kv8_rows_validate",
+    "sixi_kv8_pool_attach",
+    "sixi_kv8_attn",
+    "sixi_kv8_attn_workspace_bytes",
+    "sixi_kv8_attn_validate",
+    "sixi_rope_frequencies",
+    "sixi_qk_rope",
+    "sixi_qk_rope_validate",
+    "sixi_draft_verify",
+    "sixi_draft_workspace_bytes",
+    "sixi_draft_validate",
 )
 
 
@@ -194,6 +208,117 @@ class SixiGdnParams(ctypes.Structure):
 GDN_DECAY_FIRST = 1
 
 
+class SixiKv8Cache(ctypes.Structure):
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_exp", ctypes.c_void_p),
+        ("v_exp", ctypes.c_void_p),
+        ("k_nb", ctypes.c_int64 * 3),
+        ("v_nb", ctypes.c_int64 * 3),
+        ("k_exp_nb", ctypes.c_int64 * 3),
+        ("v_exp_nb", ctypes.c_int64 * 3),
+        ("head_dim", ctypes.c_int32),
+        ("n_heads", ctypes.c_int32),
+        ("n_blocks", ctypes.c_int64),
+        ("n", ctypes.c_int64),
+    ]
+
+
+class SixiKv8RowsParams(ctypes.Structure):
+    _fields_ = [
+        ("k", SixiView),
+        ("v", SixiView),
+        ("cache", SixiKv8Cache),
+        ("kv_len", ctypes.c_void_p),
+        ("q_len", ctypes.c_void_p),
+        ("flags", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("stream", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+    ]
+
+
+class SixiKv8AttnParams(ctypes.Structure):
+    _fields_ = [
+        ("q", SixiView),
+        ("cache", SixiKv8Cache),
+        ("out", SixiView),
+        ("kv_len", ctypes.c_void_p),
+        ("q_len", ctypes.c_void_p),
+        ("mask_mode", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+        ("mask", SixiView),
+        ("scale", ctypes.c_float),
+        ("reserved_f", ctypes.c_float),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("stream", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+    ]
+
+
+class SixiRopeScaling(ctypes.Structure):
+    _fields_ = [
+        ("kind", ctypes.c_int32),
+        ("trained_len", ctypes.c_int32),
+        ("factor", ctypes.c_double),
+        ("beta_fast", ctypes.c_double),
+        ("beta_slow", ctypes.c_double),
+    ]
+
+
+class SixiQkRopeParams(ctypes.Structure):
+    _fields_ = [
+        ("q", SixiView),
+        ("k", SixiView),
+        ("q_out", SixiView),
+        ("k_out", SixiView),
+        ("freqs", ctypes.c_void_p),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("mscale", ctypes.c_float),
+        ("n_rot", ctypes.c_int32),
+        ("layout", ctypes.c_int32),
+        ("flags", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("kv_len", ctypes.c_void_p),
+        ("pos", ctypes.c_void_p),
+        ("pos_stride", ctypes.c_int64),
+        ("q_len", ctypes.c_void_p),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+class SixiDraftParams(ctypes.Structure):
+    _fields_ = [
+        ("logits", SixiView),
+        ("draft_probs", SixiView),
+        ("draft", ctypes.c_void_p),
+        ("draft_stride", ctypes.c_int64),
+        ("u", ctypes.c_void_p),
+        ("u_stride", ctypes.c_int64),
+        ("u_next", ctypes.c_void_p),
+        ("temperature", ctypes.c_void_p),
+        ("q_len", ctypes.c_void_p),
+        ("keep", ctypes.c_void_p),
+        ("token", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("flags", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("stream", ctypes.c_void_p),
+    ]
+
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_INVERSE = 1  # flag
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_YARN = 0, 1, 2
+
+
 class SixiVerifyStream(ctypes.Structure):
     _fields_ = [("stream", ctypes.c_int32), ("cached", ctypes.c_int32), ("real", ctypes.c_int32)]
 
@@ -267,6 +392,25 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
     lib.sixi_attn_gate.restype = ctypes.c_int
     lib.sixi_gdn_verify.argtypes = [ctypes.POINTER(SixiGdnParams)]
     lib.sixi_gdn_verify.restype = ctypes.c_int
+    PN = ctypes.POINTER(ctypes.c_size_t)
+    for name, args in (
+            ("sixi_kv8_write", [ctypes.POINTER(SixiKv8RowsParams)]),
+            ("sixi_kv8_read", [ctypes.POINTER(SixiKv8RowsParams)]),
+            ("sixi_kv8_rows_validate", [ctypes.POINTER(SixiKv8RowsParams), ctypes.c_int]),
+            ("sixi_kv8_pool_attach", [vp, ctypes.POINTER(SixiKv8Cache)]),
+            ("sixi_kv8_attn", [ctypes.POINTER(SixiKv8AttnParams)]),
+            ("sixi_kv8_attn_workspace_bytes", [ctypes.POINTER(SixiKv8AttnParams), PN]),
+            ("sixi_kv8_attn_validate", [ctypes.POINTER(SixiKv8AttnParams)]),
+            ("sixi_rope_frequencies", [i32, ctypes.c_double, ctypes.POINTER(SixiRopeScaling),
+                                       ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_float)]),
+            ("sixi_qk_rope", [ctypes.POINTER(SixiQkRopeParams)]),
+            ("sixi_qk_rope_validate", [ctypes.POINTER(SixiQkRopeParams)]),
+            ("sixi_draft_verify", [ctypes.POINTER(SixiDraftParams)]),
+            ("sixi_draft_workspace_bytes", [ctypes.POINTER(SixiDraftParams), PN]),
+            ("sixi_draft_validate", [ctypes.POINTER(SixiDraftParams)])):
+        fn = getattr(lib, name)
+        fn.argtypes = args
+        fn.restype = ctypes.c_int
     if path is None:
         _lib = lib
     return lib
@@ -758,3 +902,339 @@ def gdn_verify(q, k, v, alpha, beta, y, state_in, state_out=None, q_len=None, sn
     if check and rc != OK:
         raise SixiAttnError(rc, strerror(rc))
     return rc
+
+
+# ---- around an 8-bit cache: rotary positions, store, attention, draft verification ----
+
+def _on_device(tensors, stream):
+    """The one GPU of the tensors and the stream to run on, as a handle.  Tensors (None is skipped) on several
+    devices, or on the host, raise.  Where that GPU is not the current one, the caller has to make it so
+    (:func:`_launch`)."""
+    import torch
+
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError("expected tensors on a GPU")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    return dev, (stream if stream is not None else torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _launch(fn, p, dev, check) -> int:
+    import torch
+
+    if dev.index == torch.cuda.current_device():
+        rc = fn(ctypes.byref(p))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(ctypes.byref(p))
+    if check and rc != OK:
+        raise SixiAttnError(rc, strerror(rc))
+    return rc
+
+
+def _i32(t, n: int, what: str):
+    """Address of a contiguous int32 tensor of at least n values, None for None."""
+    import torch
+
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{what}: expected {n} contiguous int32 values")
+    return t.data_ptr()
+
+
+def _f32(t, n: int, what: str):
+    import torch
+
+    if t is None:
+        return None
+    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"{what}: expected {n} contiguous float32 values")
+    return t.data_ptr()
+
+
+def _table(p, page_table, streams: int) -> None:
+    import torch
+
+    if page_table is None:
+        return
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] < streams or (
+            page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise ValueError("page_table: expected int32 [streams, pages], rows contiguous")
+    # (a stream has stride(0) pages: a row that is a part of a wider table's would reach the rest of it)
+    if page_table.shape[0] > 1 and page_table.stride(0) != page_table.shape[1]:
+        raise ValueError("page_table: expected a contiguous tensor")
+    p.page_table = page_table.data_ptr()
+    p.page_table_stride = page_table.shape[1]
+
+
+KV8_BLOCK = 32            # cells that share a scale (SIXI_KV8_BLOCK_CELLS)
+KV8_EXP_MIN, KV8_EXP_MAX = -40, 40
+
+
+class Kv8Cache:
+    """K and V of one layer in 8 bits (include/sixi_kv8.h): int8 codes and, for each block of 32 cells of a head,
+    the exponent of a power-of-two scale.
+
+    ``k[N, Hkv, blocks, D/16, 32, 16]`` and ``v[N, Hkv, blocks, D, 32]`` int8, ``k_exp/v_exp[N, Hkv, blocks]`` int8;
+    N is the streams, or the pages of a pool (then blocks is 8).  The blocks lie at any strides; each is
+    contiguous.  :meth:`empty` allocates one.  Rows go in and out with :func:`kv8_write` and :func:`kv8_read`."""
+
+    def __init__(self, k, k_exp, v, v_exp):
+        import torch
+
+        if any(t.dtype != torch.int8 for t in (k, k_exp, v, v_exp)):
+            raise ValueError("expected int8 tensors")
+        n, heads, blocks, d = v.shape[:4] if v.dim() == 5 else (0, 0, 0, 0)
+        if (v.dim() != 5 or tuple(k.shape) != (n, heads, blocks, d // 16, KV8_BLOCK, 16) or v.shape[4] != KV8_BLOCK
+                or tuple(k_exp.shape) != (n, heads, blocks) or tuple(v_exp.shape) != (n, heads, blocks)):
+            raise ValueError("expected k[N, Hkv, blocks, D/16, 32, 16], v[N, Hkv, blocks, D, 32], exponents[N, Hkv, blocks]")
+        if d not in (128, 256):
+            raise ValueError("head dim 128 or 256")
+        if tuple(k.stride()[3:]) != (512, 16, 1) or tuple(v.stride()[3:]) != (32, 1):
+            raise ValueError("a block's codes must be contiguous")
+        dev, _ = _on_device((k, k_exp, v, v_exp), 0)
+        self.k, self.k_exp, self.v, self.v_exp = k, k_exp, v, v_exp
+        self.device, self.head_dim, self.n_heads, self.n_blocks, self.n = dev, d, heads, blocks, n
+        c = self.params = SixiKv8Cache()
+        c.k, c.v, c.k_exp, c.v_exp = k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr()
+        for name, t in (("k_nb", k), ("v_nb", v), ("k_exp_nb", k_exp), ("v_exp_nb", v_exp)):
+            s = t.stride()
+            setattr(c, name, (ctypes.c_int64 * 3)(s[2], s[1], s[0]))
+        c.head_dim, c.n_heads, c.n_blocks, c.n = d, heads, blocks, n
+
+    @classmethod
+    def empty(cls, n: int, n_cells: int, n_heads: int, head_dim: int, device=None) -> "Kv8Cache":
+        """``n`` streams of ``n_cells`` cells (a multiple of 32), or ``n`` pages with ``n_cells`` = 256.  Codes of
+        zero; cells hold nothing until they are written."""
+        import torch
+
+        if n_cells % KV8_BLOCK:
+            raise ValueError("n_cells: expected a multiple of 32")
+        device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+        b = n_cells // KV8_BLOCK
+
+        def zeros(*shape):
+            return torch.zeros((n, n_heads, b, *shape), dtype=torch.int8, device=device)
+
+        return cls(zeros(head_dim // 16, KV8_BLOCK, 16), zeros(), zeros(head_dim, KV8_BLOCK), zeros())
+
+    def attach(self, pool: KvPool) -> None:
+        """Registers a cache of pages with the pool, whose copy-on-write then copies codes and exponents."""
+        rc = pool.lib.sixi_kv8_pool_attach(pool.h, ctypes.byref(self.params))
+        if rc != OK:
+            raise SixiAttnError(rc, strerror(rc))
+        pool._views.append(self)
+
+
+def _kv8_rows(fn, k, v, cache, kv_len, q_len, stream, check, page_table) -> int:
+    dev, st = _on_device((k, v, kv_len, q_len, page_table), stream)
+    if dev != cache.device:
+        raise ValueError(f"tensors on {dev}, the cache on {cache.device}")
+    p = SixiKv8RowsParams()
+    p.k, p.v = view_of(k), view_of(v)
+    p.cache = cache.params
+    s = k.shape[0]
+    p.kv_len, p.q_len = _i32(kv_len, s, "kv_len"), _i32(q_len, s, "q_len")
+    p.stream = st
+    _table(p, page_table, s)
+    return _launch(fn, p, dev, check)
+
+
+def kv8_write(k, v, cache: Kv8Cache, kv_len=None, q_len=None, stream=None, check=True, page_table=None) -> int:
+    """Stores the rows ``k/v[S, n_rows, Hkv, D]`` (f32 or f16) of each stream in cells kv_len[s] + j of an 8-bit
+    cache: each touched block's scale is the smallest power of two that holds its new rows and, where it keeps
+    cells in front of them, not below its own; kept codes are rounded to the new scale (include/sixi_kv8.h).
+    With ``page_table`` (int32 [S, pages]) the cache is a page pool.  Asynchronous on the current stream."""
+    return _kv8_rows(load_library().sixi_kv8_write, k, v, cache, kv_len, q_len, stream, check, page_table)
+
+
+def kv8_read(cache: Kv8Cache, k, v, kv_len=None, q_len=None, stream=None, check=True, page_table=None) -> int:
+    """Reads cells kv_len[s] + j of an 8-bit cache into rows j < q_len[s] of ``k/v[S, n_rows, Hkv, D]`` (f32 or
+    f16); the other rows are left as they are."""
+    return _kv8_rows(load_library().sixi_kv8_read, k, v, cache, kv_len, q_len, stream, check, page_table)
+
+
+class _Workspace:
+    """A device buffer that grows on demand and keeps what it outgrew (graphs captured over earlier calls still
+    write there), as FlashAttnExt's."""
+
+    def __init__(self, device=None):
+        import torch
+
+        self.lib = load_library()
+        self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self._ws = None
+        self._retired = []
+
+    def _give(self, p, size_of, workspace) -> int:
+        import torch
+
+        n = ctypes.c_size_t(0)
+        rc = size_of(ctypes.byref(p), ctypes.byref(n))
+        if rc != OK:
+            return rc
+        ws = workspace
+        if ws is None:
+            ws = self._ws
+            if ws is None or ws.numel() < n.value:
+                if ws is not None:
+                    self._retired.append(ws)
+                ws = self._ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
+        p.workspace = ws.data_ptr()
+        p.workspace_bytes = ws.numel() * ws.element_size()
+        return OK
+
+
+class Kv8Attention(_Workspace):
+    """Attention over an 8-bit cache (include/sixi_kv8.h): one token, a drafted block or a prompt chunk per stream.
+
+    Keeps a device workspace, as :class:`FlashAttnExt` does: calls of one object must be ordered on one stream, and
+    so must graphs captured over it; calls that may overlap take an object each (or a ``workspace`` each)."""
+
+    def params(self, q, cache: Kv8Cache, out, kv_len=None, q_len=None, mask_mode=MASK_BLOCK_CAUSAL, mask=None, scale=None,
+               page_table=None) -> SixiKv8AttnParams:
+        p = SixiKv8AttnParams()
+        p.q, p.out = view_of(q), view_of(out, tokens_heads=False)
+        p.cache = cache.params
+        s = q.shape[0]
+        p.kv_len, p.q_len = _i32(kv_len, s, "kv_len"), _i32(q_len, s, "q_len")
+        p.mask_mode = mask_mode
+        if mask is not None:
+            p.mask = view_of(mask, tokens_heads=False)
+        p.scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+        _table(p, page_table, s)
+        return p
+
+    def workspace_bytes(self, p: SixiKv8AttnParams) -> int:
+        n = ctypes.c_size_t(0)
+        rc = self.lib.sixi_kv8_attn_workspace_bytes(ctypes.byref(p), ctypes.byref(n))
+        if rc != OK:
+            raise SixiAttnError(rc, strerror(rc))
+        return n.value
+
+    def __call__(self, q, cache: Kv8Cache, out, kv_len=None, q_len=None, mask_mode=MASK_BLOCK_CAUSAL, mask=None, scale=None,
+                 stream=None, check=True, workspace=None, page_table=None) -> int:
+        """``q[S, n_q, H, D]`` f16 or f32, ``out[S, n_q, H, D]`` f32 or f16; ``mask`` (MASK_EXPLICIT) f16
+        ``[S or 1, 1, >= n_q, n_kv]``; ``page_table`` int32 [S, pages]: the cache is a page pool.  Rows past q_len are
+        not written; a row that sees no cell is zero."""
+        dev, st = _on_device((q, out, kv_len, q_len, mask, page_table, workspace), stream)
+        if dev != cache.device or dev != self.device:
+            raise ValueError(f"tensors on {dev}, the cache on {cache.device}, the handle on {self.device}")
+        p = self.params(q, cache, out, kv_len, q_len, mask_mode, mask, scale, page_table)
+        p.stream = st
+        rc = self._give(p, self.lib.sixi_kv8_attn_workspace_bytes, workspace)
+        if rc != OK:
+            if check:
+                raise SixiAttnError(rc, strerror(rc))
+            return rc
+        return _launch(self.lib.sixi_kv8_attn, p, dev, check)
+
+
+def rope_frequencies(n_rot: int, base: float, scaling: int = ROPE_SCALE_NONE, factor: float = 1.0, trained_len: int = 0,
+                     beta_fast: float = 32.0, beta_slow: float = 1.0, device=None):
+    """(freqs, mscale) for :func:`qk_rope`: the radians per position of each pair as a float64 tensor on ``device``
+    (the current GPU), and the factor on the rotated values (include/sixi_rope.h ``sixi_rope_frequencies``)."""
+    import torch
+
+    sc = SixiRopeScaling(scaling, trained_len, factor, beta_fast, beta_slow)
+    f, m = (ctypes.c_double * max(1, n_rot // 2))(), ctypes.c_float(0)
+    rc = load_library().sixi_rope_frequencies(n_rot, base, ctypes.byref(sc), f, ctypes.byref(m))
+    if rc != OK:
+        raise SixiAttnError(rc, strerror(rc))
+    return torch.tensor(f[:n_rot // 2], dtype=torch.float64, device="cuda" if device is None else device), m.value
+
+
+def qk_rope(q, k, freqs, q_out=None, k_out=None, kv_len=None, pos=None, q_len=None, layout: int = ROPE_HALF,
+            mscale: float = 1.0, q_norm=None, k_norm=None, eps: float = 1e-6, inverse: bool = False, stream=None,
+            check=True) -> int:
+    """Rotary positions of ``q[S, n_rows, H, D]`` and ``k[S, n_rows, Hkv, D]`` (or None) into ``q_out`` and ``k_out``
+    (None: in place), f32 or f16 each (include/sixi_rope.h).
+
+    ``freqs`` float64 [n_rot/2] radians per position (:func:`rope_frequencies`); row j of stream s stands at
+    ``pos[s, j]`` (int32), or at kv_len[s] + j.  ``q_norm/k_norm`` (f32 [D]): an RMS norm first.  ``inverse`` turns
+    back.  Rows past q_len are left as they are.  Asynchronous on the current stream."""
+    import torch
+
+    dev, st = _on_device((q, k, freqs, q_out, k_out, kv_len, pos, q_len, q_norm, k_norm), stream)
+    if freqs.dtype != torch.float64 or not freqs.is_contiguous():
+        raise ValueError("freqs: expected contiguous float64 values")
+    p = SixiQkRopeParams()
+    s, n, d = q.shape[0], q.shape[1], q.shape[3]
+    p.q = view_of(q, tokens_heads=False)
+    p.q_out = view_of(q if q_out is None else q_out, tokens_heads=False)
+    if k is not None:
+        p.k = view_of(k, tokens_heads=False)
+        p.k_out = view_of(k if k_out is None else k_out, tokens_heads=False)
+    p.freqs, p.n_rot = freqs.data_ptr(), 2 * freqs.numel()
+    p.q_norm, p.k_norm = _f32(q_norm, d, "q_norm"), _f32(k_norm, d, "k_norm")
+    p.eps, p.mscale, p.layout = eps, mscale, layout
+    if inverse:
+        p.flags = ROPE_INVERSE
+    p.kv_len, p.q_len = _i32(kv_len, s, "kv_len"), _i32(q_len, s, "q_len")
+    if pos is not None:
+        if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[0] < s or pos.shape[1] < n or (n > 1 and pos.stride(1) != 1):
+            raise ValueError("pos: expected int32 [S, n_rows], rows contiguous")
+        p.pos, p.pos_stride = pos.data_ptr(), pos.stride(0)
+    p.stream = st
+    return _launch(load_library().sixi_qk_rope, p, dev, check)
+
+
+def _rows_view(t) -> SixiView:
+    """View [V, rows, S, 1] of a (S, rows, V) tensor of logits or probabilities."""
+    import torch
+
+    kind = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}.get(t.dtype)
+    if kind is None or t.dim() != 3:
+        raise ValueError("expected f32, f16 or bf16 [S, rows, V]")
+    es, (s, n, v), (b2, b1, b0) = t.element_size(), t.shape, t.stride()
+    return SixiView.from_buffer_copy(_VIEW.pack(t.data_ptr(), kind, 0, v, n, s, 1, b0 * es, b1 * es, b2 * es, 0))
+
+
+class DraftVerify(_Workspace):
+    """Which drafted tokens stay, and the token behind them (include/sixi_draft.h).
+
+    Keeps a device workspace: calls of one object must be ordered on one stream, as :class:`Kv8Attention`'s."""
+
+    def params(self, logits, draft, u, u_next, keep, token, draft_probs=None, q_len=None, temperature=None) -> SixiDraftParams:
+        import torch
+
+        p = SixiDraftParams()
+        s, n = logits.shape[:2]
+        p.logits = _rows_view(logits)
+        if draft_probs is not None and n > 1:
+            p.draft_probs = _rows_view(draft_probs)
+        if n > 1:
+            for t, kind, what in ((draft, torch.int32, "draft: expected int32"), (u, torch.float32, "u: expected float32")):
+                if t is None or t.dtype != kind or t.dim() != 2 or t.shape[0] < s or t.shape[1] < n - 1 or (n > 2 and t.stride(1) != 1):
+                    raise ValueError(what + " [S, rows - 1], rows contiguous")
+            p.draft, p.draft_stride = draft.data_ptr(), draft.stride(0)
+            p.u, p.u_stride = u.data_ptr(), u.stride(0)
+        p.u_next, p.temperature = _f32(u_next, s, "u_next"), _f32(temperature, s, "temperature")
+        p.q_len, p.keep, p.token = _i32(q_len, s, "q_len"), _i32(keep, s, "keep"), _i32(token, s, "token")
+        return p
+
+    def __call__(self, logits, draft, u, u_next, keep, token, draft_probs=None, q_len=None, temperature=None, stream=None,
+                 check=True, workspace=None) -> int:
+        """``logits[S, rows, V]`` of the target, row j for what follows row j; ``draft[S, rows - 1]`` int32 the drafted
+        tokens, ``draft_probs[S, rows - 1, V]`` what they were drawn from (None: drafted without chance);
+        ``u[S, rows - 1]`` and ``u_next[S]`` f32 in [0, 1); ``q_len[S]`` rows of each stream (1 + drafts);
+        ``temperature[S]`` f32, 0 for greedy.  Writes ``keep[S]`` (rows that stay: 1 + tokens kept, what the GDN's
+        ``snap`` takes) and ``token[S]`` int32."""
+        dev, st = _on_device((logits, draft, u, u_next, keep, token, draft_probs, q_len, temperature, workspace), stream)
+        if dev != self.device:
+            raise ValueError(f"tensors on {dev}, the handle on {self.device}")
+        p = self.params(logits, draft, u, u_next, keep, token, draft_probs, q_len, temperature)
+        p.stream = st
+        rc = self._give(p, self.lib.sixi_draft_workspace_bytes, workspace)
+        if rc != OK:
+            if check:
+                raise SixiAttnError(rc, strerror(rc))
+            return rc
+        return _launch(self.lib.sixi_draft_verify, p, dev, check)
