@@ -43,7 +43,8 @@ HIP_FLAGS = [
 # the chunked kernel's state, which is an MFMA operand and accumulator at once (in AGPR form it
 # took 52 AGPRs and 244 VGPRs).
 FILE_FLAGS = {"fa_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
-              "gdn_verify.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]}
+              "gdn_verify.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"],
+              "kv8_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=true"]}
 
 
 def flags_for(src: str) -> list[str]:

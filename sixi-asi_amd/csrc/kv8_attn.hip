@@ -7,27 +7,43 @@
 // it lies in memory: 16 bytes per lane, 1 KiB per wave.  Codes become f16 exactly (|code| <= 127), the
 // scales are powers of two and never meet an element:
 //   t = scale log2(e) 2^ek (q . k) + ev        the exponent of (weight * 2^ev)
-//   P' = 2^(t - m)                              m the running maximum of t (less kHead)
+//   P' = 2^(t - m)                              m a reference near the running maximum of t
 //   O' = sum P' v,   l = sum P' 2^-ev,   o = O' / l
 // With ev inside the exponent a block's V scale costs nothing, and the f16 rounding of P' is half a step
 // of 11 bits of each weight, down to 2^-24 of the largest contribution whatever the blocks' scales are.
-// l is summed from the unrounded weights in f32.
+// l is the f32 sum of the same f16 weights.
 //
 // The cell that score register i of a lane holds is ours to choose (any order of K's rows will do):
 // lane (n, h) of the 32 x 32 result holds cells 16h .. 16h + 15 of the block in order, which is what the
 // lane needs as its half of the next product's right operand.  So P never leaves its lane.
+//
+// Two kernels.  Up to 32 rows a group (decode): the four waves of a work-group take blocks in turn,
+// straight from memory into registers, one block ahead; nothing is shared.  More rows: NW waves take 32
+// rows each of the same cells; a step's codes are converted once, by all of them, into f16 operands in
+// LDS (two buffers, the next step's codes on their way in registers).
+//
+// Work-groups: every stream's cells are cut into pieces of c blocks, c from the lengths on the device, so
+// that streams of any lengths fill the chip; pieces of one (stream, head, tile) are joined by a second
+// launch in their order.
+#include <type_traits>
+
+#include "device_util.hpp"
 #include "kv8_device.hpp"
 
 namespace sixi {
 namespace {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8u __attribute__((ext_vector_type(8), aligned(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLowest = -3e38f;  // below every score: the running maximum of a row that has seen no cell
-// The largest weight is 2^kHead, not 1: f16 weights keep 11 bits down to 2^-24 of it.
-constexpr float kHead = 10.0f;
+constexpr float kLowest = -3e38f;  // below every score: the reference of a row that has seen no cell
+// The largest weight stands between 2^kHead and 2^kRoof: f16 weights keep 11 bits down to 2^-24 of 2^kHead,
+// and the accumulators are rescaled only when a maximum has grown by 2^(kRoof - kHead).
+constexpr float kHead = 10.0f, kRoof = 15.0f;
 
 // Four int8 codes as f16, exactly: the code + 128 under the exponent of 1024, less 1152.
 __device__ __forceinline__ void codes_f16(uint32_t c, f16x2& lo, f16x2& hi) {
@@ -64,21 +80,87 @@ __device__ __forceinline__ Lens lens_of(const Kv8AttnArgs& a, int s) {
     r.cells = r.cached + r.rows;  // (without kv_len: all n_kv)
     return r;
 }
+__device__ __forceinline__ int blocks_of(const Lens& n) { return (n.cells + kBlk - 1) / kBlk; }
 
-// Blocks [first, last) of piece `i` of `n` of a stream.
-__device__ __forceinline__ void piece_of(int cells, int i, int n, int& first, int& last) {
-    const int blocks = (cells + kBlk - 1) / kBlk, each = (blocks + n - 1) / n;
-    first = min(i * each, blocks);
-    last = min(first + each, blocks);
-}
+// How a call's cells are cut: pieces of c blocks, numbered stream by stream.  c is the work of
+// all streams over the work-groups asked for; nothing is cut where the tiles alone are nearly enough of
+// them.  Whole numbers, formed alike by every work-group of a call and of its merge.
+struct Place {
+    int s, tiles, pieces, at;  // stream, its tiles, pieces of each, number of its first piece
+};
+struct Cut {
+    int c, total;
+    // of the lane's stream (S <= 64), else of the last 64 looked at
+    int tiles, pieces, at, mine;
 
-__device__ __forceinline__ float* slot_of(const Kv8AttnArgs& a, int s, int g, int tile, int piece) {
-    return a.part + ((((int64_t)s * a.Hkv + g) * a.n_tiles + tile) * a.n_split + piece) * (32 * (int64_t)a.D + 64);
-}
+    __device__ __forceinline__ void stream(const Kv8AttnArgs& a, int s, int& t, int& blocks) const {
+        t = blocks = 0;
+        if (s < a.S) {
+            const Lens n = lens_of(a, s);
+            t = (n.rows * a.G + 32 * a.waves - 1) / (32 * a.waves);
+            blocks = blocks_of(n);
+        }
+    }
+    __device__ __forceinline__ void count(const Kv8AttnArgs& a, int t, int blocks, int before) {
+        tiles = t;
+        pieces = max(1, (blocks + c - 1) / c);
+        mine = t * pieces * a.Hkv;
+        const int run = wave_scan(mine);
+        at = before + run - mine;
+        total = before + __builtin_amdgcn_readlane(run, 63);
+    }
+    __device__ __forceinline__ void begin(const Kv8AttnArgs& a) {
+        const int lane = threadIdx.x & 63;
+        int t = 0, blocks = 0, all = 0, work = 0;
+        for (int s0 = 0; s0 < a.S; s0 += 64) {
+            stream(a, s0 + lane, t, blocks);
+            // (a stream's share of a work-group's blocks, in 1/64: 2^21 blocks of 2^15 tiles stay in range)
+            all += __builtin_amdgcn_readlane(wave_scan(t), 63);
+            work += __builtin_amdgcn_readlane(wave_scan((int)min((int64_t)t * blocks * a.Hkv * 64 / a.target + 1, (int64_t)1 << 22)), 63);
+        }
+        c = (int64_t)all * a.Hkv * 4 >= (int64_t)a.target * 3 ? 1 << 26 : (max((work + 63) / 64, a.least) + 1) / 2 * 2;  // (even: two blocks a step, and of one page)
+        total = 0;
+        if (a.S <= 64)
+            count(a, t, blocks, 0);
+        else
+            for (int s0 = 0; s0 < a.S; s0 += 64) {
+                stream(a, s0 + lane, t, blocks);
+                count(a, t, blocks, total);
+            }
+    }
+    // The stream that holds piece `id`, or (by_stream) the place of stream `id`.
+    __device__ __forceinline__ Place find(const Kv8AttnArgs& a, int id, bool by_stream) {
+        const int lane = threadIdx.x & 63, sum = total;
+        Place p{0, 1, 1, 0};
+        int before = 0;
+        for (int s0 = 0; s0 < a.S; s0 += 64) {
+            if (a.S > 64) {
+                int t, blocks;
+                stream(a, s0 + lane, t, blocks);
+                count(a, t, blocks, before);
+                before = total;
+            }
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(by_stream ? s0 + lane == id : id >= at && id < at + mine);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                p.s = s0 + l;
+                p.tiles = __builtin_amdgcn_readlane(tiles, l);
+                p.pieces = __builtin_amdgcn_readlane(pieces, l);
+                p.at = __builtin_amdgcn_readlane(at, l);
+                break;
+            }
+        }
+        total = sum;
+        return p;
+    }
+};
+
+// Floats of a piece's partial result: per wave-tile of 32 rows, O in the order of the accumulators
+// [D/8][64 lanes][4], then m and l of 32 rows.
+__device__ __host__ constexpr int64_t tile_floats(int D) { return 32 * (int64_t)D + 64; }
 
 __device__ __forceinline__ void store4(const Kv8AttnArgs& a, char* row, int d, kv8_f32x4 x) {
     if (a.o_f16) {
-        typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
         f16x4 h;
 #pragma unroll
         for (int i = 0; i < 4; ++i) h[i] = (_Float16)x[i];
@@ -88,243 +170,491 @@ __device__ __forceinline__ void store4(const Kv8AttnArgs& a, char* row, int d, k
     }
 }
 
-constexpr int kWaves = 4;
-
-template <int D, bool MASK>
-__global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_kernel(Kv8AttnArgs a) {
-    constexpr int KC = D / 32;  // 32-dim pieces of a row: K loads, V loads and output tiles
-    extern __shared__ __align__(16) float lds[];
-    const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int piece = blockIdx.x % a.n_split, tile = blockIdx.x / a.n_split, g = blockIdx.y, s = blockIdx.z;
-    const Lens len = lens_of(a, s);
-    const int M = len.rows * a.G;
-    if (tile * 32 >= M) return;
-    int b0, b1;
-    piece_of(len.cells, piece, a.n_split, b0, b1);
-    if (b0 >= b1 && piece > 0) return;
-
-    // the lane's row: its query, and the last cell that it sees
-    const int r = tile * 32 + n;
-    const bool live = r < M;
-    const int j = live ? r / a.G : 0, head = live ? g * a.G + r % a.G : g * a.G;
-    const int last = a.mode == SIXI_MASK_BLOCK_CAUSAL ? len.cached + j : len.cells - 1;
-    const int sees = a.mode == SIXI_MASK_BLOCK_CAUSAL ? len.cached + tile * 32 / a.G : len.cells - 1;  // by every row
-    // cells behind the last that any row of the tile sees are not read
-    const int jl = (min(tile * 32 + 32, M) - 1) / a.G;
-    const int reach = a.mode == SIXI_MASK_BLOCK_CAUSAL ? len.cached + jl + 1 : len.cells;
-    b1 = min(b1, (reach + kBlk - 1) / kBlk);
+// What a wave holds: 32 rows of a group, their queries and sums.
+template <int D>
+struct Rows {
+    static constexpr int KC = D / 32;  // 32-dim pieces of a row: K loads, V loads and output tiles
     kv8_f16x8 q[KC][2];
-    {
+    f32x16 o[KC];
+    float m, l;
+    int last;     // the last cell that the lane's row sees
+    int sees;     // the last cell that every row sees
+    int reach;    // cells that any of the rows sees
+    int j, head;
+    bool live;
+
+    __device__ __forceinline__ void begin(const Kv8AttnArgs& a, const Lens& n, int s, int g, int r0) {
+        const int lane = threadIdx.x & 63, M = n.rows * a.G, r = r0 + (lane & 31), h = lane >> 5;
+        live = r < M;
+        j = live ? r / a.G : 0;
+        head = live ? g * a.G + r % a.G : g * a.G;
+        const bool causal = a.mode == SIXI_MASK_BLOCK_CAUSAL;
+        last = causal ? n.cached + j : n.cells - 1;
+        sees = causal ? n.cached + r0 / a.G : n.cells - 1;
+        reach = causal ? n.cached + (min(r0 + 32, M) - 1) / a.G + 1 : n.cells;
+        if (r0 >= M) reach = 0;
         const char* p = a.q + (int64_t)j * a.q_nb1 + (int64_t)head * a.q_nb2 + (int64_t)s * a.q_nb3;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int d = (2 * c + h) * 16 + 8 * u;
-                kv8_f16x8 x;
-                if (a.q_f16) {
-                    x = *reinterpret_cast<const kv8_f16x8*>(p + d * 2);
-                } else {
-                    const kv8_f32x4 lo = *reinterpret_cast<const kv8_f32x4*>(p + d * 4);
-                    const kv8_f32x4 hi = *reinterpret_cast<const kv8_f32x4*>(p + d * 4 + 16);
+                kv8_f16x8 x = {};
+                if (live) {
+                    if (a.q_f16) {
+                        x = *reinterpret_cast<const kv8_f16x8*>(p + d * 2);
+                    } else {
+                        const kv8_f32x4 lo = *reinterpret_cast<const kv8_f32x4*>(p + d * 4);
+                        const kv8_f32x4 hi = *reinterpret_cast<const kv8_f32x4*>(p + d * 4 + 16);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[i] = (_Float16)lo[i];
-                        x[4 + i] = (_Float16)hi[i];
+                        for (int i = 0; i < 4; ++i) {
+                            x[i] = (_Float16)lo[i];
+                            x[4 + i] = (_Float16)hi[i];
+                        }
                     }
+                    x = x * (_Float16)a.q_sign;
                 }
-                const _Float16 sign = (_Float16)(live ? a.q_sign : 0.0f);
-                q[c][u] = live ? x * sign : kv8_f16x8{};
+                q[c][u] = x;
             }
+#pragma unroll
+        for (int c = 0; c < KC; ++c) o[c] = f32x16{};
+        m = kLowest;
+        l = 0.0f;
     }
-    const char* mask = nullptr;
-    if (MASK) mask = a.mask + (int64_t)j * a.m_nb1 + (int64_t)s * a.m_nb3;
 
-    f32x16 o[KC];
-#pragma unroll
-    for (int c = 0; c < KC; ++c) o[c] = f32x16{};
-    float m = kLowest, l = 0.0f;
-    const int k_off = h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
-    const int v_off = n * kBlk + h * 16;
-
-    for (int b = b0 + wave; b < b1; b += kWaves) {
-        int64_t k_at, ke_at, v_at, ve_at;
-        block_at(a.pages, a.k.nb, a.k.e_nb, s, b, k_at, ke_at);
-        block_at(a.pages, a.v.nb, a.v.e_nb, s, b, v_at, ve_at);
-        const char* kp = a.k.codes + k_at + (int64_t)g * a.k.nb[1];
-        const char* vp = a.v.codes + v_at + (int64_t)g * a.v.nb[1];
-        kv8_u32x4 kc[KC], vc[KC];
-#pragma unroll
-        for (int c = 0; c < KC; ++c) kc[c] = *reinterpret_cast<const kv8_u32x4*>(kp + k_off + c * (kBlk * 32));
-#pragma unroll
-        for (int c = 0; c < KC; ++c) vc[c] = *reinterpret_cast<const kv8_u32x4*>(vp + v_off + c * (kBlk * 32));
-        const int ek = clamp_exp(a.k.exps[ke_at + (int64_t)g * a.k.e_nb[1]]);
-        const int ev = clamp_exp(a.v.exps[ve_at + (int64_t)g * a.v.e_nb[1]]);
-
-        f32x16 sc = {};
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            kv8_f16x8 x, y;
-            codes_f16x16(kc[c], x, y);
-            sc = mfma(x, q[c][0], sc);
-            sc = mfma(y, q[c][1], sc);
-        }
-        const float ks = a.scale_log2 * exp2_int(ek), es = (float)ev;
-        const int cell0 = b * kBlk + 16 * h;
-        float top;
+    // A block's scores: hidden cells to -inf; with a mask, to t itself.
+    template <bool MASK>
+    __device__ __forceinline__ void hide(const Kv8AttnArgs& a, f32x16& sc, int block, float ks, float es, const char* mask) const {
+        const int cell0 = block * kBlk + 16 * ((threadIdx.x & 63) >> 5);
         if (MASK) {
+            f16x8u add[2];
+            if (block * kBlk + kBlk - 1 <= last) {
+                add[0] = *reinterpret_cast<const f16x8u*>(mask + (int64_t)cell0 * 2);
+                add[1] = *reinterpret_cast<const f16x8u*>(mask + (int64_t)cell0 * 2 + 16);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float add = -__builtin_huge_valf();
-                if (cell0 + i <= last) add = (float)*reinterpret_cast<const _Float16*>(mask + (int64_t)(cell0 + i) * 2);
-                sc[i] = fmaf(sc[i], ks, fmaf(add, kLog2e, es));
+                for (int i = 0; i < 16; ++i) {
+                    _Float16 x = (_Float16)-__builtin_huge_valf();
+                    if (cell0 + i <= last) x = *reinterpret_cast<const _Float16*>(mask + (int64_t)(cell0 + i) * 2);
+                    add[i / 8][i % 8] = x;
+                }
             }
-            top = sc[0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
-        } else {
-            if (b * kBlk + kBlk - 1 > sees) {
+            for (int i = 0; i < 16; ++i) sc[i] = fmaf(sc[i], ks, fmaf((float)add[i / 8][i % 8], kLog2e, es));
+        } else if (block * kBlk + kBlk - 1 > sees) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (cell0 + i > last) sc[i] = -__builtin_huge_valf();
-            }
-            top = sc[0];
-#pragma unroll
-            for (int i = 1; i < 16; ++i) top = fmaxf(top, sc[i]);
-            top = fmaf(top, ks, es);
+            for (int i = 0; i < 16; ++i)
+                if (cell0 + i > last) sc[i] = -__builtin_huge_valf();
         }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float up = fmaxf(m, top - kHead);
-        if (__builtin_amdgcn_ballot_w64(up > m)) {
-            const float f = __builtin_amdgcn_exp2f(m - up);
+    }
+    // The row's largest t of a block (maxima that keep NaN: no operand is canonicalised first).
+    template <bool MASK>
+    __device__ __forceinline__ float top_of(const f32x16& sc, float ks, float es) const {
+        float top = __builtin_elementwise_maximum(sc[0], sc[1]), top2 = __builtin_elementwise_maximum(sc[2], sc[3]);
+#pragma unroll
+        for (int i = 4; i < 16; i += 4) {
+            top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top, sc[i]), sc[i + 1]);
+            top2 = __builtin_elementwise_maximum(__builtin_elementwise_maximum(top2, sc[i + 2]), sc[i + 3]);
+        }
+        top = max_halves(__builtin_elementwise_maximum(top, top2));
+        return MASK ? top : fmaf(top, ks, es);
+    }
+    // A new reference where a maximum has outgrown the old one (a NaN has not; its weights are NaN).
+    __device__ __forceinline__ void raise(float top) {
+        const bool grow = top > m + kRoof;
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+            const float up = grow ? top - kHead : m, f = __builtin_amdgcn_exp2f(m - up);
             m = up;
             l *= f;
 #pragma unroll
             for (int c = 0; c < KC; ++c) o[c] *= f;
         }
+    }
+    // Scores to weights in f16, and their sum.
+    template <bool MASK>
+    __device__ __forceinline__ void weights(const f32x16& sc, float ks, float es, int ev, kv8_f16x8 (&p)[2]) {
         const float sub = MASK ? -m : es - m;
-        float sum = 0.0f;
-        kv8_f16x8 p[2];
+        const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float w = __builtin_amdgcn_exp2f(MASK ? sc[i] + sub : fmaf(sc[i], ks, sub));
-            sum += w;
-            p[i / 8][i % 8] = (_Float16)w;
-        }
-        l = fmaf(sum, exp2_int(-ev), l);
+        for (int i = 0; i < 16; i += 2) {
+            f32x2 w;
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            kv8_f16x8 x, y;
-            codes_f16x16(vc[c], x, y);
-            o[c] = mfma(x, p[0], o[c]);
-            o[c] = mfma(y, p[1], o[c]);
+            for (int e = 0; e < 2; ++e) w[e] = __builtin_amdgcn_exp2f(MASK ? sc[i + e] + sub : fmaf(sc[i + e], ks, sub));
+            const f16x2 x = __builtin_convertvector(w, f16x2);
+            p[i / 8][i % 8] = x[0];
+            p[i / 8][i % 8 + 1] = x[1];
+            sum[i / 2 % 2] = __builtin_amdgcn_fdot2(x, one, sum[i / 2 % 2], false);
         }
+        l = fmaf(sum[0] + sum[1], exp2_int(-ev), l);
     }
-    l += __shfl_xor(l, 32, 64);
 
-    // the waves' results into the first one's, two and then one at a time
-    for (int half = kWaves / 2; half > 0; half /= 2) {
-        float* buf = lds + (wave % half) * (32 * D + 64);
-        if (wave >= half && wave < 2 * half) {
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) buf[(c * 16 + i) * 64 + lane] = o[c][i];
-            if (h == 0) {
-                buf[32 * D + n] = m;
-                buf[32 * D + 32 + n] = l;
-            }
-        }
-        __syncthreads();
-        if (wave < half) {
-            const float m2 = buf[32 * D + n], l2 = buf[32 * D + 32 + n], up = fmaxf(m, m2);
-            const float f = __builtin_amdgcn_exp2f(m - up), f2 = __builtin_amdgcn_exp2f(m2 - up);
-            m = up;
-            l = l * f + l2 * f2;
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[c][i] = o[c][i] * f + buf[(c * 16 + i) * 64 + lane] * f2;
-        }
-        __syncthreads();
-    }
-    if (wave != 0 || !live) return;
-    if (a.n_split == 1) {
+    __device__ __forceinline__ void finish(const Kv8AttnArgs& a, int s) {
+        if (!live) return;
+        const int h = (threadIdx.x & 63) >> 5;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         char* row = a.out + (int64_t)head * a.o_nb1 + (int64_t)j * a.o_nb2 + (int64_t)s * a.o_nb3;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                store4(a, row, c * 32 + 2 * i + 4 * h,
-                       kv8_f32x4{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]} * inv);
-    } else {
-        float* part = slot_of(a, s, g, tile, piece);
+                store4(a, row, c * 32 + 2 * i + 4 * h, kv8_f32x4{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]} * inv);
+    }
+
+    // Another wave's sums of the same rows, as leave() wrote them.
+    __device__ __forceinline__ void join(const float* part) {
+        const int lane = threadIdx.x & 63, n = lane & 31;
+        if (!live) return;
+        const float m2 = part[32 * D + n], l2 = part[32 * D + 32 + n], up = fmaxf(m, m2);
+        const float f = __builtin_amdgcn_exp2f(m - up), f2 = __builtin_amdgcn_exp2f(m2 - up);
+        m = up;
+        l = l * f + l2 * f2;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const kv8_f32x4 x = *reinterpret_cast<const kv8_f32x4*>(part + ((c * 4 + i / 4) * 64 + lane) * 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[c][i + e] = o[c][i + e] * f + x[e] * f2;
+            }
+    }
+
+    __device__ __forceinline__ void leave(float* part) {
+        const int lane = threadIdx.x & 63;
+        if (!live) return;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<kv8_f32x4*>(part + n * D + c * 32 + 2 * i + 4 * h) =
+                *reinterpret_cast<kv8_f32x4*>(part + ((c * 4 + i / 4) * 64 + lane) * 4) =
                     kv8_f32x4{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]};
-        if (h == 0) {
-            part[32 * D + n] = m;
-            part[32 * D + 32 + n] = l;
+        if (lane < 32) {
+            part[32 * D + lane] = m;
+            part[32 * D + 32 + lane] = l;
         }
     }
+};
+
+// The piece of a work-group, in the order (stream, tile from the last on, piece, head): the longest tiles of a
+// causal chunk first, and, as work-groups go round the 8 XCDs, tiles of the same head on few of them, where
+// they meet in the L2.
+struct Work {
+    int s, g, tile, id, first, last, pieces;
+    Lens n;
+};
+__device__ __forceinline__ bool work_of(const Kv8AttnArgs& a, Work& w) {
+    Cut cut;
+    cut.begin(a);
+    w.id = blockIdx.x;
+    if (w.id >= cut.total) return false;
+    const Place p = cut.find(a, w.id, false);
+    w.s = p.s;
+    w.pieces = p.pieces;
+    const int x = w.id - p.at;
+    w.g = x % a.Hkv;
+    const int y = x / a.Hkv, piece = y % p.pieces;
+    w.tile = p.tiles - 1 - y / p.pieces;
+    w.n = lens_of(a, w.s);
+    w.first = piece * cut.c;
+    w.last = min(blocks_of(w.n), w.first + cut.c);
+    return true;
 }
 
-// One work-group per (stream, kv-head, tile): a row's pieces in their order.
+constexpr int kWaves = 4;
+
+template <int D, bool MASK>
+__global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_kernel(Kv8AttnArgs a) {
+    constexpr int KC = D / 32;
+    extern __shared__ __align__(16) float lds[];
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Work w;
+    if (!work_of(a, w)) return;
+    Rows<D> r;
+    r.begin(a, w.n, w.s, w.g, w.tile * 32);
+    const char* mask = MASK ? a.mask + (int64_t)r.j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
+    const int last = min(w.last, (r.reach + kBlk - 1) / kBlk);
+    const uint32_t k_off = h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
+    const uint32_t v_off = n * kBlk + h * 16;
+
+    // K of the next block is asked for when this one's is f16, V when this one's is spent
+    int b = w.first + wave;
+    if (b < last) {
+        kv8_u32x4 kc[KC], vc[KC];
+        BlockWalk walk;
+        walk.begin(a.pages, a.k, a.v, w.s, w.g, b, last);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.k + k_off + c * (kBlk * 32));
+        int ek = *walk.ke, ev = *walk.ve;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) vc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.v + v_off + c * (kBlk * 32));
+        walk.go(a.pages, a.k, a.v, w.s, w.g, kWaves);
+        for (; b < last; b += kWaves) {
+            f32x16 sc = {};
+            kv8_f16x8 x[KC][2];
+#pragma unroll
+            for (int c = 0; c < KC; ++c) codes_f16x16(kc[c], x[c][0], x[c][1]);
+            const int ek0 = clamp_exp(ek), ev0 = clamp_exp(ev);
+#pragma unroll
+            for (int c = 0; c < KC; ++c) kc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.k + k_off + c * (kBlk * 32));
+            ek = *walk.ke;
+            ev = *walk.ve;
+            const char* vn = walk.v;
+            walk.go(a.pages, a.k, a.v, w.s, w.g, kWaves);
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                sc = mfma(x[c][0], r.q[c][0], sc);
+                sc = mfma(x[c][1], r.q[c][1], sc);
+            }
+            kv8_f16x8 p[2];
+            const float ks = a.scale_log2 * exp2_int(ek0), es = (float)ev0;
+            r.template hide<MASK>(a, sc, b, ks, es, mask);
+            r.raise(r.template top_of<MASK>(sc, ks, es));
+            r.template weights<MASK>(sc, ks, es, ev0, p);
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                kv8_f16x8 y[2];
+                codes_f16x16(vc[c], y[0], y[1]);
+                vc[c] = *reinterpret_cast<const kv8_u32x4*>(vn + v_off + c * (kBlk * 32));
+                r.o[c] = mfma(y[0], p[0], r.o[c]);
+                r.o[c] = mfma(y[1], p[1], r.o[c]);
+            }
+        }
+    }
+    r.l = sum_halves(r.l);
+
+    // the waves' results into the first one's, two and then one at a time
+    for (int half = kWaves / 2; half > 0; half /= 2) {
+        float* buf = lds + (wave % half) * tile_floats(D);
+        if (wave >= half && wave < 2 * half) r.leave(buf);
+        __syncthreads();
+        if (wave < half) r.join(buf);
+        __syncthreads();
+    }
+    if (wave != 0) return;
+    if (w.pieces == 1)
+        r.finish(a, w.s);
+    else
+        r.leave(a.part + w.id * tile_floats(D));
+}
+
+// Four waves of 32 rows each over the same cells, NB blocks of 32 a step.  A wave without rows still converts
+// its share of the codes: three waves of rows and one without measured faster than a work-group of three.
+template <int D, int NB>
+constexpr size_t rows_lds() {
+    return (size_t)2 * 2 * NB * (D / 32) * 2 * 64 * 16;
+}
+
+template <int D, int NB, bool MASK>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnArgs a) {
+    constexpr int NW = kWaves;
+    constexpr int KC = D / 32, ITEMS = NB * KC, MINE = (ITEMS + NW - 1) / NW;
+    extern __shared__ __align__(16) float lds[];
+    // [buffer][K, V][block, piece][first, second eight][lane] 8 f16
+    typedef kv8_f16x8 Tile[2][ITEMS][2][64];
+    Tile* tile = reinterpret_cast<Tile*>(lds);
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Work w;
+    if (!work_of(a, w)) return;
+    const int r0 = w.tile * (32 * NW);
+    Rows<D> r;
+    r.begin(a, w.n, w.s, w.g, r0 + wave * 32);
+    const char* mask = MASK ? a.mask + (int64_t)r.j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
+    int last = w.last;  // blocks that any row of the work-group sees
+    if (a.mode == SIXI_MASK_BLOCK_CAUSAL)
+        last = min(last, (w.n.cached + (min(r0 + 32 * NW, w.n.rows * a.G) - 1) / a.G + kBlk) / kBlk);
+    if (w.first < last) {
+        const uint32_t k_off = h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
+        const uint32_t v_off = n * kBlk + h * 16;
+        // the wave's share of the next step's codes, on their way
+        kv8_u32x4 kc[MINE], vc[MINE];
+        int ek[NB], ev[NB];
+        BlockWalk walk;
+        auto fetch = [&](kv8_u32x4 (&codes)[MINE], const char* p, uint32_t off, int32_t step) {
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+                const int it = min(wave + i * NW, ITEMS - 1);
+                codes[i] = *reinterpret_cast<const kv8_u32x4*>(p + ((NB > 1 && it >= KC ? step : 0) + it % KC * (kBlk * 32)) + off);
+            }
+        };
+        // the walk's step; a second block that is none is the first once more (its cells are hidden).  The
+        // compiler is not to know that: it would wait for the first one's exponents to copy them.
+        auto load = [&]() {
+            const bool both = walk.b + 1 < last;
+            int k_step = both ? walk.k_nb : 0, v_step = both ? walk.v_nb : 0;
+            int ke_step = both ? walk.ke_nb : 0, ve_step = both ? walk.ve_nb : 0;
+            asm("" : "+s"(k_step), "+s"(v_step), "+s"(ke_step), "+s"(ve_step));
+            fetch(kc, walk.k, k_off, k_step);
+            fetch(vc, walk.v, v_off, v_step);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                ek[i] = walk.ke[i * ke_step];
+                ev[i] = walk.ve[i * ve_step];
+            }
+            walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
+        };
+        float ks[NB], es[NB];
+        int e0[NB];
+        // the codes as f16 into a buffer
+        auto convert = [&](int buf) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < MINE; ++i) {
+                    const int it = wave + i * NW;
+                    if (ITEMS % NW == 0 || it < ITEMS) {
+                        kv8_f16x8 x, y;
+                        codes_f16x16(k ? vc[i] : kc[i], x, y);
+                        tile[buf][k][it][0][lane] = x;
+                        tile[buf][k][it][1][lane] = y;
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+                ks[i] = a.scale_log2 * exp2_int(clamp_exp(ek[i]));
+                e0[i] = clamp_exp(ev[i]);
+                es[i] = (float)e0[i];
+            }
+        };
+        // One step.  EDGE: some row may not see every cell.  The products run at a raised priority, so that
+        // the matrix cores serve one wave of a SIMD while the other is at its softmax.
+        auto step = [&](int b, auto BUF, auto EDGE) {
+            constexpr int buf = decltype(BUF)::value;
+            load();  // (behind the last step: its blocks once more, and not used)
+            if (!decltype(EDGE)::value || b * kBlk < r.reach) {
+                f32x16 sc[NB] = {};
+                kv8_f16x8 p[NB][2];
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) {
+                        sc[i] = mfma(tile[buf][0][i * KC + c][0][lane], r.q[c][0], sc[i]);
+                        sc[i] = mfma(tile[buf][0][i * KC + c][1][lane], r.q[c][1], sc[i]);
+                    }
+                __builtin_amdgcn_s_setprio(0);
+                float top = kLowest;
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                    if (decltype(EDGE)::value) r.template hide<MASK>(a, sc[i], b + i, ks[i], es[i], mask);
+                    top = __builtin_elementwise_maximum(top, r.template top_of<MASK>(sc[i], ks[i], es[i]));
+                }
+                r.raise(top);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) r.template weights<MASK>(sc[i], ks[i], es[i], e0[i], p[i]);
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int i = 0; i < NB; ++i)
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) {
+                        r.o[c] = mfma(tile[buf][1][i * KC + c][0][lane], p[i][0], r.o[c]);
+                        r.o[c] = mfma(tile[buf][1][i * KC + c][1][lane], p[i][1], r.o[c]);
+                    }
+                __builtin_amdgcn_s_setprio(0);
+            }
+            convert(buf ^ 1);
+            __syncthreads();
+        };
+        walk.begin(a.pages, a.k, a.v, w.s, w.g, w.first, last);
+        load();
+        convert(0);
+        __syncthreads();
+        // steps in pairs, one for each buffer; first those whose cells every row of the work-group sees
+        using std::integral_constant;
+        const int sees = a.mode == SIXI_MASK_BLOCK_CAUSAL ? w.n.cached + r0 / a.G + 1 : w.n.cells;
+        const int plain = MASK || r0 + 32 * NW > w.n.rows * a.G ? w.first : min(last, sees / kBlk);
+        int b = w.first;
+#pragma unroll 1
+        for (; b + 2 * NB <= plain; b += 2 * NB) {
+            step(b, integral_constant<int, 0>{}, integral_constant<bool, false>{});
+            step(b + NB, integral_constant<int, 1>{}, integral_constant<bool, false>{});
+        }
+#pragma unroll 1
+        for (; b < last; b += 2 * NB) {
+            step(b, integral_constant<int, 0>{}, integral_constant<bool, true>{});
+            if (b + NB < last) step(b + NB, integral_constant<int, 1>{}, integral_constant<bool, true>{});
+        }
+    }
+    r.l = sum_halves(r.l);
+    if (w.pieces == 1)
+        r.finish(a, w.s);
+    else
+        r.leave(a.part + ((int64_t)w.id * NW + wave) * tile_floats(D));
+}
+
+// Joins the pieces of 32 rows: D/32 work-groups of 256 threads, each with 4 of the accumulators' D/8 quads.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a) {
-    const int tile = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
+    const int s = blockIdx.z, g = blockIdx.y, quads = blockIdx.x % (D / 32), t32 = blockIdx.x / (D / 32);
+    Cut cut;
+    cut.begin(a);
+    const Place p = cut.find(a, s, true);
     const Lens len = lens_of(a, s);
     const int M = len.rows * a.G;
-    if (tile * 32 >= M) return;
-    const int blocks = (len.cells + kBlk - 1) / kBlk, each = (blocks + a.n_split - 1) / a.n_split;
-    const int pieces = each > 0 ? (blocks + each - 1) / each : 1;
-    for (int x = threadIdx.x; x < 32 * D / 4; x += blockDim.x) {
-        const int n = x / (D / 4), d = x % (D / 4) * 4, r = tile * 32 + n;
-        if (r >= M) continue;
-        const float* p = slot_of(a, s, g, tile, 0);
-        const int64_t stride = 32 * (int64_t)D + 64;
-        float m = kLowest;
-        for (int i = 0; i < pieces; ++i) m = fmaxf(m, p[i * stride + 32 * D + n]);
-        float l = 0.0f;
-        kv8_f32x4 o = {};
-        for (int i = 0; i < pieces; ++i) {
-            const float f = __builtin_amdgcn_exp2f(p[i * stride + 32 * D + n] - m);
-            l = fmaf(p[i * stride + 32 * D + 32 + n], f, l);
-            o += *reinterpret_cast<const kv8_f32x4*>(p + i * stride + n * D + d) * f;
-        }
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        const int j = r / a.G, head = g * a.G + r % a.G;
-        store4(a, a.out + (int64_t)head * a.o_nb1 + (int64_t)j * a.o_nb2 + (int64_t)s * a.o_nb3, d, o * inv);
+    if (t32 * 32 >= M || p.pieces == 1) return;
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, quad = quads * 4 + (threadIdx.x >> 6);
+    const int rr = t32 * 32 + n;
+    if (rr >= M) return;
+    const int64_t step = (int64_t)a.Hkv * a.waves * tile_floats(D);  // from piece to piece
+    const float* at = a.part + (((int64_t)p.at + (int64_t)(p.tiles - 1 - t32 / a.waves) * p.pieces * a.Hkv + g) * a.waves + t32 % a.waves) * tile_floats(D);
+    float m = kLowest;
+#pragma unroll 4
+    for (int i = 0; i < p.pieces; ++i) m = fmaxf(m, at[i * step + 32 * D + n]);
+    float l = 0.0f;
+    kv8_f32x4 o = {};
+#pragma unroll 4
+    for (int i = 0; i < p.pieces; ++i) {
+        const float f = __builtin_amdgcn_exp2f(at[i * step + 32 * D + n] - m);
+        l = fmaf(at[i * step + 32 * D + 32 + n], f, l);
+        o += *reinterpret_cast<const kv8_f32x4*>(at + i * step + (quad * 64 + lane) * 4) * f;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const int j = rr / a.G, head = g * a.G + rr % a.G;
+    store4(a, a.out + (int64_t)head * a.o_nb1 + (int64_t)j * a.o_nb2 + (int64_t)s * a.o_nb3, quad / 4 * 32 + quad % 4 * 8 + 4 * h, o * inv);
+}
+
+template <int D, bool MASK>
+void launch_pieces(const Kv8AttnArgs& a, hipStream_t stream) {
+    if (a.waves == 1) {
+        const size_t lds = (size_t)(kWaves / 2) * tile_floats(D) * sizeof(float);
+        hipLaunchKernelGGL((kv8_attn_few_kernel<D, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
+    } else {
+        constexpr int NB = D == 128 ? 2 : 1;
+        constexpr size_t lds = rows_lds<D, NB>();
+        hipLaunchKernelGGL((kv8_attn_rows_kernel<D, NB, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
     }
 }
 
 template <int D>
 hipError_t launch(const Kv8AttnArgs& a, hipStream_t stream) {
-    const dim3 grid((unsigned)(a.n_tiles * a.n_split), (unsigned)a.Hkv, (unsigned)a.S);
-    const size_t lds = (size_t)(kWaves / 2) * kv8_slot_floats(D) * sizeof(float);
     if (a.mode == SIXI_MASK_EXPLICIT)
-        hipLaunchKernelGGL((kv8_attn_kernel<D, true>), grid, dim3(kWaves * 64), lds, stream, a);
+        launch_pieces<D, true>(a, stream);
     else
-        hipLaunchKernelGGL((kv8_attn_kernel<D, false>), grid, dim3(kWaves * 64), lds, stream, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.n_split == 1) return e;
-    hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3((unsigned)a.n_tiles, (unsigned)a.Hkv, (unsigned)a.S), dim3(256), 0, stream, a);
+        launch_pieces<D, false>(a, stream);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !a.cut) return e;
+    const int64_t t32 = ((int64_t)a.n_q * a.G + 31) / 32;
+    hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3((unsigned)(t32 * (D / 32)), (unsigned)a.Hkv, (unsigned)a.S), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
 }  // namespace
 
-// Two rounds of work-groups, in pieces of at least 8 blocks (two steps of a wave).
-int kv8_attn_splits(int64_t S, int64_t Hkv, int64_t tiles, int64_t n_kv) {
-    const int64_t groups = S * Hkv * tiles, blocks = (n_kv + kBlk - 1) / kBlk;
-    int64_t n = (512 + groups - 1) / groups;
-    if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
-    return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+size_t kv8_attn_plan(Kv8AttnArgs& a) {
+    const int64_t t32 = ((int64_t)a.n_q * a.G + 31) / 32;
+    a.waves = t32 == 1 ? 1 : kWaves;
+    a.target = 2 * device_cu_count();
+    a.least = a.waves == 1 ? 8 : 4;
+    const int64_t tiles = (t32 + a.waves - 1) / a.waves * a.Hkv * a.S;
+    const int64_t blocks = (a.n_kv + kBlk - 1) / kBlk;
+    // pieces at most: one for each tile, and those that a cut makes (the last few: the round-robin over 8
+    // XCDs, and f32 sums of large numbers); a cut is made only over fewer tiles than 3/4 of the target
+    a.cut = blocks > a.least;
+    a.grid = (int32_t)(tiles + (a.cut ? a.target : 0) + 16);
+    if (!a.cut) return 256;
+    const int64_t slots = (tiles < a.target ? tiles : a.target) + a.target + 16;
+    return ((size_t)slots * a.waves * tile_floats(a.D) * sizeof(float) + 255) / 256 * 256;
 }
 
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t stream) {

@@ -62,14 +62,16 @@ struct Kv8AttnArgs {
     float scale_log2;             // |scale| * log2(e); the sign goes into Q
     float q_sign;
     float* part;                  // workspace
-    int32_t n_split, n_tiles;     // pieces of a stream's cells, 32-row tiles of a group's rows
+    int32_t waves;                // row tiles of 32 that a work-group takes (1: its waves share the cells)
+    int32_t target;               // work-groups that the cells are cut for
+    int32_t least;                // blocks of a piece at least
+    int32_t grid;                 // pieces at most
+    int32_t cut;                  // whether cells may be cut (partial results in the workspace)
 };
 
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t stream);
 
-// Pieces that a stream's cells are cut into.
-int kv8_attn_splits(int64_t S, int64_t Hkv, int64_t tiles, int64_t n_kv);
-// f32 values of the partial results of one (piece, tile).
-inline int64_t kv8_slot_floats(int D) { return 32 * (int64_t)D + 64; }
+// Chooses waves, target, least and grid for the shape; the workspace's bytes.
+size_t kv8_attn_plan(Kv8AttnArgs& a);
 
 }  // namespace sixi

@@ -44,6 +44,8 @@ int check_cache(const sixi_kv8_cache& c, bool paged, CacheViews* out) {
     for (int i = 0; i < 3; ++i) {
         if (c.k_nb[i] < 0 || c.v_nb[i] < 0 || c.k_exp_nb[i] < 0 || c.v_exp_nb[i] < 0) return SIXI_E_INVALID_ARGUMENT;
         if (c.k_nb[i] % 16 || c.v_nb[i] % 16) return SIXI_E_ALIGNMENT;
+        if (i == 0 && (c.k_nb[0] > INT32_MAX || c.v_nb[0] > INT32_MAX || c.k_exp_nb[0] > INT32_MAX || c.v_exp_nb[0] > INT32_MAX))
+            return SIXI_E_UNSUPPORTED;  // (steps from block to block are 32-bit)
     }
     if (!aligned(c.k, 16) || !aligned(c.v, 16)) return SIXI_E_ALIGNMENT;
     const int64_t bytes = (int64_t)sixi::kBlk * c.head_dim;
@@ -222,11 +224,8 @@ int resolve_attn(const sixi_kv8_attn_params* p, sixi::Kv8AttnArgs* out, size_t* 
     // a scale of 0 becomes one that no score can notice: hidden cells are -inf times it
     a.scale_log2 = std::fmax(std::fabs(p->scale) * 1.4426950408889634f, 0x1p-85f);
     a.q_sign = std::signbit(p->scale) ? -1.0f : 1.0f;
-    a.n_tiles = (int32_t)((a.n_q * (int64_t)a.G + 31) / 32);
-    a.n_split = sixi::kv8_attn_splits(S, a.Hkv, a.n_tiles, n_kv);
-    *ws = 256;
-    if (a.n_split > 1)
-        *ws = ((size_t)(S * a.Hkv * (int64_t)a.n_tiles * a.n_split * sixi::kv8_slot_floats(a.D)) * sizeof(float) + 255) / 256 * 256;
+    if ((a.n_q * (int64_t)a.G + 31) / 32 * a.Hkv * S > ((int64_t)1 << 28)) return SIXI_E_UNSUPPORTED;  // work-groups
+    *ws = sixi::kv8_attn_plan(a);
     a.part = static_cast<float*>(p->workspace);
     *out = a;
     return SIXI_OK;
