@@ -17,6 +17,7 @@ GPU before a pass; buffers and the calls' handles are kept from pass to pass.
 """
 from __future__ import annotations
 
+import functools
 import math
 import pathlib
 import sys
@@ -31,6 +32,7 @@ EPS = 1e-6
 E_MIN, E_MAX = -40, 40  # range of a block's scale exponent
 
 
+@functools.lru_cache(maxsize=None)
 def _framework():
     root = str(pathlib.Path(__file__).resolve().parents[1] / "sixi-asi_amd")
     if root not in sys.path:
