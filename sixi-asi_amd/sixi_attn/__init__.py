@@ -905,73 +905,130 @@ def gdn_verify(q, k, v, alpha, beta, y, state_in, state_out=None, q_len=None, sn
 
 
 # ---- around an 8-bit cache: rotary positions, store, attention, draft verification ----
+#
+# These calls are made once per layer and token, so their host path counts: a call's C struct is packed at once
+# (struct.Struct of the whole layout) and handed over as bytes.
 
-def _on_device(tensors, stream):
-    """The one GPU of the tensors and the stream to run on, as a handle.  Tensors (None is skipped) on several
-    devices, or on the host, raise.  Where that GPU is not the current one, the caller has to make it so
-    (:func:`_launch`)."""
+@functools.lru_cache(maxsize=None)
+def _torch():
     import torch
 
-    dev = None
-    for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("expected tensors on a GPU")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    return dev, (stream if stream is not None else torch.cuda.current_stream(dev).cuda_stream)
+    return torch
 
 
-def _launch(fn, p, dev, check) -> int:
-    import torch
-
-    if dev.index == torch.cuda.current_device():
-        rc = fn(ctypes.byref(p))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(p))
-    if check and rc != OK:
-        raise SixiAttnError(rc, strerror(rc))
-    return rc
+@functools.lru_cache(maxsize=None)
+def _kinds() -> dict:
+    torch = _torch()
+    return {torch.float32: (TYPE_F32, 4), torch.float16: (TYPE_F16, 2), torch.bfloat16: (TYPE_BF16, 2)}
 
 
-def _i32(t, n: int, what: str):
-    """Address of a contiguous int32 tensor of at least n values, None for None."""
-    import torch
+_NO_VIEW = (0,) * 11
+_V = "Qii8q"  # a SixiView
 
+
+def _kind(t, what: str):
+    try:
+        return _kinds()[t.dtype]
+    except KeyError:
+        raise ValueError(f"{what}: unexpected type {t.dtype}") from None
+
+
+def _rows4(t, what: str):
+    """View [D, tokens, heads, S] of a (S, tokens, heads, D) tensor, as the values of a SixiView."""
+    kind, es = _kind(t, what)
+    try:
+        s, n, h, d = t.shape
+    except ValueError:
+        raise ValueError(f"{what}: expected a 4-d tensor") from None
+    b3, b1, b2, b0 = t.stride()
+    return t.data_ptr(), kind, 0, d, n, h, s, b0 * es, b1 * es, b2 * es, b3 * es
+
+
+def _plain4(t, what: str):
+    """View of a 4-d tensor with its dims reversed."""
+    kind, es = _kind(t, what)
+    try:
+        n3, n2, n1, n0 = t.shape
+    except ValueError:
+        raise ValueError(f"{what}: expected a 4-d tensor") from None
+    b3, b2, b1, b0 = t.stride()
+    return t.data_ptr(), kind, 0, n0, n1, n2, n3, b0 * es, b1 * es, b2 * es, b3 * es
+
+
+def _rows3(t, what: str):
+    """View [V, rows, S, 1] of a (S, rows, V) tensor."""
+    kind, es = _kind(t, what)
+    try:
+        s, n, v = t.shape
+    except ValueError:
+        raise ValueError(f"{what}: expected [S, rows, V]") from None
+    b2, b1, b0 = t.stride()
+    return t.data_ptr(), kind, 0, v, n, s, 1, b0 * es, b1 * es, b2 * es, 0
+
+
+def _i32(t, n: int, what: str) -> int:
+    """Address of a contiguous int32 tensor of at least n values, 0 for None."""
     if t is None:
-        return None
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
+        return 0
+    if t.dtype is not _torch().int32 or not t.is_contiguous() or t.numel() < n:
         raise ValueError(f"{what}: expected {n} contiguous int32 values")
     return t.data_ptr()
 
 
-def _f32(t, n: int, what: str):
-    import torch
-
+def _f32(t, n: int, what: str) -> int:
     if t is None:
-        return None
-    if t.dtype != torch.float32 or not t.is_contiguous() or t.numel() < n:
+        return 0
+    if t.dtype is not _torch().float32 or not t.is_contiguous() or t.numel() < n:
         raise ValueError(f"{what}: expected {n} contiguous float32 values")
     return t.data_ptr()
 
 
-def _table(p, page_table, streams: int) -> None:
-    import torch
+def _table(t, streams: int):
+    """(address, entries of a row) of a page table."""
+    if t is None:
+        return 0, 0
+    if t.dtype is not _torch().int32 or t.dim() != 2 or t.shape[0] < streams or not t.is_contiguous():
+        raise ValueError("page_table: expected contiguous int32 [streams, pages]")
+    return t.data_ptr(), t.shape[1]
 
-    if page_table is None:
-        return
-    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] < streams or (
-            page_table.shape[1] > 1 and page_table.stride(1) != 1):
-        raise ValueError("page_table: expected int32 [streams, pages], rows contiguous")
-    # (a stream has stride(0) pages: a row that is a part of a wider table's would reach the rest of it)
-    if page_table.shape[0] > 1 and page_table.stride(0) != page_table.shape[1]:
-        raise ValueError("page_table: expected a contiguous tensor")
-    p.page_table = page_table.data_ptr()
-    p.page_table_stride = page_table.shape[1]
+
+def _device_of(first, *more) -> int:
+    """The index of the GPU that every tensor is on (None is skipped)."""
+    dev = first.get_device()
+    if dev < 0:
+        raise ValueError("expected tensors on a GPU")
+    for t in more:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {first.device} and {t.device}")
+    return dev
+
+
+def _stream_of(stream, dev: int) -> int:
+    return _torch()._C._cuda_getCurrentRawStream(dev) if stream is None else stream
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    """An entry point that takes its struct as bytes."""
+    fn = load_library()[name]
+    fn.argtypes = [ctypes.c_char_p]
+    fn.restype = ctypes.c_int
+    return fn
+
+
+def _launch(fn, packed: bytes, dev: int) -> int:
+    """Runs an entry point with the tensors' GPU as the current one."""
+    torch = _torch()
+    if dev == torch._C._cuda_getDevice():
+        return fn(packed)
+    with torch.cuda.device(dev):
+        return fn(packed)
+
+
+def _checked(rc: int, check: bool) -> int:
+    if check and rc != OK:
+        raise SixiAttnError(rc, strerror(rc))
+    return rc
 
 
 KV8_BLOCK = 32            # cells that share a scale (SIXI_KV8_BLOCK_CELLS)
@@ -999,15 +1056,16 @@ class Kv8Cache:
             raise ValueError("head dim 128 or 256")
         if tuple(k.stride()[3:]) != (512, 16, 1) or tuple(v.stride()[3:]) != (32, 1):
             raise ValueError("a block's codes must be contiguous")
-        dev, _ = _on_device((k, k_exp, v, v_exp), 0)
+        self.device_index = _device_of(k, k_exp, v, v_exp)
         self.k, self.k_exp, self.v, self.v_exp = k, k_exp, v, v_exp
-        self.device, self.head_dim, self.n_heads, self.n_blocks, self.n = dev, d, heads, blocks, n
+        self.head_dim, self.n_heads, self.n_blocks, self.n = d, heads, blocks, n
         c = self.params = SixiKv8Cache()
         c.k, c.v, c.k_exp, c.v_exp = k.data_ptr(), v.data_ptr(), k_exp.data_ptr(), v_exp.data_ptr()
         for name, t in (("k_nb", k), ("v_nb", v), ("k_exp_nb", k_exp), ("v_exp_nb", v_exp)):
-            s = t.stride()
-            setattr(c, name, (ctypes.c_int64 * 3)(s[2], s[1], s[0]))
+            st = t.stride()
+            setattr(c, name, (ctypes.c_int64 * 3)(st[2], st[1], st[0]))
         c.head_dim, c.n_heads, c.n_blocks, c.n = d, heads, blocks, n
+        self.packed = bytes(c)
 
     @classmethod
     def empty(cls, n: int, n_cells: int, n_heads: int, head_dim: int, device=None) -> "Kv8Cache":
@@ -1033,18 +1091,21 @@ class Kv8Cache:
         pool._views.append(self)
 
 
-def _kv8_rows(fn, k, v, cache, kv_len, q_len, stream, check, page_table) -> int:
-    dev, st = _on_device((k, v, kv_len, q_len, page_table), stream)
-    if dev != cache.device:
-        raise ValueError(f"tensors on {dev}, the cache on {cache.device}")
-    p = SixiKv8RowsParams()
-    p.k, p.v = view_of(k), view_of(v)
-    p.cache = cache.params
+_C = f"{ctypes.sizeof(SixiKv8Cache)}s"
+_KV8_ROWS = struct.Struct("=" + _V + _V + _C + "QQiiQQq")
+_KV8_ATTN = struct.Struct("=" + _V + _C + _V + "QQii" + _V + "ffQQQQq")
+_ROPE = struct.Struct("=" + 4 * _V + "QQQffiiiiQQqQQ")
+_DRAFT = struct.Struct("=" + _V + _V + "QqQqQQQQQQQiiQ")
+for _s, _c in ((_KV8_ROWS, SixiKv8RowsParams), (_KV8_ATTN, SixiKv8AttnParams), (_ROPE, SixiQkRopeParams), (_DRAFT, SixiDraftParams)):
+    assert _s.size == ctypes.sizeof(_c), _c
+
+
+def _kv8_rows(name, k, v, cache, kv_len, q_len, stream, check, page_table) -> int:
+    dev = _device_of(k, v, kv_len, q_len, page_table, cache.k)
     s = k.shape[0]
-    p.kv_len, p.q_len = _i32(kv_len, s, "kv_len"), _i32(q_len, s, "q_len")
-    p.stream = st
-    _table(p, page_table, s)
-    return _launch(fn, p, dev, check)
+    return _checked(_launch(_entry(name), _KV8_ROWS.pack(
+        *_rows4(k, "k"), *_rows4(v, "v"), cache.packed, _i32(kv_len, s, "kv_len"), _i32(q_len, s, "q_len"), 0, 0,
+        _stream_of(stream, dev), *_table(page_table, s)), dev), check)
 
 
 def kv8_write(k, v, cache: Kv8Cache, kv_len=None, q_len=None, stream=None, check=True, page_table=None) -> int:
@@ -1052,44 +1113,57 @@ def kv8_write(k, v, cache: Kv8Cache, kv_len=None, q_len=None, stream=None, check
     cache: each touched block's scale is the smallest power of two that holds its new rows and, where it keeps
     cells in front of them, not below its own; kept codes are rounded to the new scale (include/sixi_kv8.h).
     With ``page_table`` (int32 [S, pages]) the cache is a page pool.  Asynchronous on the current stream."""
-    return _kv8_rows(load_library().sixi_kv8_write, k, v, cache, kv_len, q_len, stream, check, page_table)
+    return _kv8_rows("sixi_kv8_write", k, v, cache, kv_len, q_len, stream, check, page_table)
 
 
 def kv8_read(cache: Kv8Cache, k, v, kv_len=None, q_len=None, stream=None, check=True, page_table=None) -> int:
     """Reads cells kv_len[s] + j of an 8-bit cache into rows j < q_len[s] of ``k/v[S, n_rows, Hkv, D]`` (f32 or
     f16); the other rows are left as they are."""
-    return _kv8_rows(load_library().sixi_kv8_read, k, v, cache, kv_len, q_len, stream, check, page_table)
+    return _kv8_rows("sixi_kv8_read", k, v, cache, kv_len, q_len, stream, check, page_table)
 
 
 class _Workspace:
     """A device buffer that grows on demand and keeps what it outgrew (graphs captured over earlier calls still
     write there), as FlashAttnExt's."""
 
-    def __init__(self, device=None):
-        import torch
+    _entries = ("", "")  # the call and the size of its workspace
 
+    def __init__(self, device=None):
+        torch = _torch()
         self.lib = load_library()
         self.device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+        self.device_index = torch.cuda.current_device() if self.device.index is None else self.device.index
         self._ws = None
         self._retired = []
 
-    def _give(self, p, size_of, workspace) -> int:
-        import torch
-
+    def workspace_bytes(self, p) -> int:
+        """Bytes that a call of these parameters needs (:meth:`params`, or their bytes)."""
         n = ctypes.c_size_t(0)
-        rc = size_of(ctypes.byref(p), ctypes.byref(n))
+        p = p if isinstance(p, ctypes.Structure) else self._struct.from_buffer_copy(p)
+        rc = getattr(self.lib, self._entries[1])(ctypes.byref(p), ctypes.byref(n))
         if rc != OK:
-            return rc
-        ws = workspace
-        if ws is None:
-            ws = self._ws
-            if ws is None or ws.numel() < n.value:
-                if ws is not None:
-                    self._retired.append(ws)
-                ws = self._ws = torch.empty(n.value, dtype=torch.uint8, device=self.device)
-        p.workspace = ws.data_ptr()
-        p.workspace_bytes = ws.numel() * ws.element_size()
-        return OK
+            raise SixiAttnError(rc, strerror(rc))
+        return n.value
+
+    def _run(self, pack, dev, workspace, check) -> int:
+        """``pack(address, bytes)`` gives the call's struct with that workspace."""
+        if dev != self.device_index:
+            raise ValueError(f"tensors on GPU {dev}, the handle on {self.device_index}")
+        fn = _entry(self._entries[0])
+        if workspace is not None:
+            return _checked(_launch(fn, pack(workspace.data_ptr(), workspace.numel() * workspace.element_size()), dev), check)
+        ws = self._ws
+        rc = E_OUT_OF_BOUNDS if ws is None else _launch(fn, pack(ws.data_ptr(), ws.numel()), dev)
+        if rc == E_OUT_OF_BOUNDS:  # none yet, or too small for this call: nothing has been launched
+            try:
+                n = self.workspace_bytes(pack(0, 0))
+            except SixiAttnError as e:
+                return _checked(e.code, check)
+            if ws is not None:
+                self._retired.append(ws)
+            ws = self._ws = _torch().empty(n, dtype=_torch().uint8, device=self.device)
+            rc = _launch(fn, pack(ws.data_ptr(), n), dev)
+        return _checked(rc, check)
 
 
 class Kv8Attention(_Workspace):
@@ -1098,43 +1172,32 @@ class Kv8Attention(_Workspace):
     Keeps a device workspace, as :class:`FlashAttnExt` does: calls of one object must be ordered on one stream, and
     so must graphs captured over it; calls that may overlap take an object each (or a ``workspace`` each)."""
 
-    def params(self, q, cache: Kv8Cache, out, kv_len=None, q_len=None, mask_mode=MASK_BLOCK_CAUSAL, mask=None, scale=None,
-               page_table=None) -> SixiKv8AttnParams:
-        p = SixiKv8AttnParams()
-        p.q, p.out = view_of(q), view_of(out, tokens_heads=False)
-        p.cache = cache.params
-        s = q.shape[0]
-        p.kv_len, p.q_len = _i32(kv_len, s, "kv_len"), _i32(q_len, s, "q_len")
-        p.mask_mode = mask_mode
-        if mask is not None:
-            p.mask = view_of(mask, tokens_heads=False)
-        p.scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-        _table(p, page_table, s)
-        return p
+    _struct = SixiKv8AttnParams
+    _entries = ("sixi_kv8_attn", "sixi_kv8_attn_workspace_bytes")
 
-    def workspace_bytes(self, p: SixiKv8AttnParams) -> int:
-        n = ctypes.c_size_t(0)
-        rc = self.lib.sixi_kv8_attn_workspace_bytes(ctypes.byref(p), ctypes.byref(n))
-        if rc != OK:
-            raise SixiAttnError(rc, strerror(rc))
-        return n.value
+    @staticmethod
+    def _packer(q, cache, out, kv_len, q_len, mask_mode, mask, scale, page_table, stream):
+        s = q.shape[0]
+        head = (*_rows4(q, "q"), cache.packed, *_plain4(out, "out"), _i32(kv_len, s, "kv_len"), _i32(q_len, s, "q_len"),
+                mask_mode, 0, *(_NO_VIEW if mask is None else _plain4(mask, "mask")),
+                1.0 / math.sqrt(cache.head_dim) if scale is None else scale, 0.0)
+        tail = (stream, *_table(page_table, s))
+        return lambda at, n: _KV8_ATTN.pack(*head, at, n, *tail)
+
+    def params(self, q, cache: Kv8Cache, out, kv_len=None, q_len=None, mask_mode=MASK_BLOCK_CAUSAL, mask=None, scale=None,
+               page_table=None, stream=0) -> SixiKv8AttnParams:
+        """The call's C struct, without a workspace."""
+        return SixiKv8AttnParams.from_buffer_copy(
+            self._packer(q, cache, out, kv_len, q_len, mask_mode, mask, scale, page_table, stream)(0, 0))
 
     def __call__(self, q, cache: Kv8Cache, out, kv_len=None, q_len=None, mask_mode=MASK_BLOCK_CAUSAL, mask=None, scale=None,
                  stream=None, check=True, workspace=None, page_table=None) -> int:
         """``q[S, n_q, H, D]`` f16 or f32, ``out[S, n_q, H, D]`` f32 or f16; ``mask`` (MASK_EXPLICIT) f16
         ``[S or 1, 1, >= n_q, n_kv]``; ``page_table`` int32 [S, pages]: the cache is a page pool.  Rows past q_len are
         not written; a row that sees no cell is zero."""
-        dev, st = _on_device((q, out, kv_len, q_len, mask, page_table, workspace), stream)
-        if dev != cache.device or dev != self.device:
-            raise ValueError(f"tensors on {dev}, the cache on {cache.device}, the handle on {self.device}")
-        p = self.params(q, cache, out, kv_len, q_len, mask_mode, mask, scale, page_table)
-        p.stream = st
-        rc = self._give(p, self.lib.sixi_kv8_attn_workspace_bytes, workspace)
-        if rc != OK:
-            if check:
-                raise SixiAttnError(rc, strerror(rc))
-            return rc
-        return _launch(self.lib.sixi_kv8_attn, p, dev, check)
+        dev = _device_of(q, out, kv_len, q_len, mask, page_table, workspace, cache.k)
+        return self._run(self._packer(q, cache, out, kv_len, q_len, mask_mode, mask, scale, page_table, _stream_of(stream, dev)),
+                         dev, workspace, check)
 
 
 def rope_frequencies(n_rot: int, base: float, scaling: int = ROPE_SCALE_NONE, factor: float = 1.0, trained_len: int = 0,
@@ -1160,41 +1223,24 @@ def qk_rope(q, k, freqs, q_out=None, k_out=None, kv_len=None, pos=None, q_len=No
     ``freqs`` float64 [n_rot/2] radians per position (:func:`rope_frequencies`); row j of stream s stands at
     ``pos[s, j]`` (int32), or at kv_len[s] + j.  ``q_norm/k_norm`` (f32 [D]): an RMS norm first.  ``inverse`` turns
     back.  Rows past q_len are left as they are.  Asynchronous on the current stream."""
-    import torch
-
-    dev, st = _on_device((q, k, freqs, q_out, k_out, kv_len, pos, q_len, q_norm, k_norm), stream)
-    if freqs.dtype != torch.float64 or not freqs.is_contiguous():
+    dev = _device_of(q, k, freqs, q_out, k_out, kv_len, pos, q_len, q_norm, k_norm)
+    torch = _torch()
+    if freqs.dtype is not torch.float64 or not freqs.is_contiguous():
         raise ValueError("freqs: expected contiguous float64 values")
-    p = SixiQkRopeParams()
-    s, n, d = q.shape[0], q.shape[1], q.shape[3]
-    p.q = view_of(q, tokens_heads=False)
-    p.q_out = view_of(q if q_out is None else q_out, tokens_heads=False)
-    if k is not None:
-        p.k = view_of(k, tokens_heads=False)
-        p.k_out = view_of(k if k_out is None else k_out, tokens_heads=False)
-    p.freqs, p.n_rot = freqs.data_ptr(), 2 * freqs.numel()
-    p.q_norm, p.k_norm = _f32(q_norm, d, "q_norm"), _f32(k_norm, d, "k_norm")
-    p.eps, p.mscale, p.layout = eps, mscale, layout
-    if inverse:
-        p.flags = ROPE_INVERSE
-    p.kv_len, p.q_len = _i32(kv_len, s, "kv_len"), _i32(q_len, s, "q_len")
+    s, n, _, d = q.shape
+    pos_at = pos_stride = 0
     if pos is not None:
-        if pos.dtype != torch.int32 or pos.dim() != 2 or pos.shape[0] < s or pos.shape[1] < n or (n > 1 and pos.stride(1) != 1):
+        if pos.dtype is not torch.int32 or pos.dim() != 2 or pos.shape[0] < s or pos.shape[1] < n or (n > 1 and pos.stride(1) != 1):
             raise ValueError("pos: expected int32 [S, n_rows], rows contiguous")
-        p.pos, p.pos_stride = pos.data_ptr(), pos.stride(0)
-    p.stream = st
-    return _launch(load_library().sixi_qk_rope, p, dev, check)
-
-
-def _rows_view(t) -> SixiView:
-    """View [V, rows, S, 1] of a (S, rows, V) tensor of logits or probabilities."""
-    import torch
-
-    kind = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}.get(t.dtype)
-    if kind is None or t.dim() != 3:
-        raise ValueError("expected f32, f16 or bf16 [S, rows, V]")
-    es, (s, n, v), (b2, b1, b0) = t.element_size(), t.shape, t.stride()
-    return SixiView.from_buffer_copy(_VIEW.pack(t.data_ptr(), kind, 0, v, n, s, 1, b0 * es, b1 * es, b2 * es, 0))
+        pos_at, pos_stride = pos.data_ptr(), pos.stride(0)
+    vq = _plain4(q, "q")
+    vk = _NO_VIEW if k is None else _plain4(k, "k")
+    packed = _ROPE.pack(
+        *vq, *vk, *(vq if q_out is None else _plain4(q_out, "q_out")),
+        *(vk if k is None or k_out is None else _plain4(k_out, "k_out")), freqs.data_ptr(), _f32(q_norm, d, "q_norm"),
+        _f32(k_norm, d, "k_norm"), eps, mscale, 2 * freqs.numel(), layout, ROPE_INVERSE if inverse else 0, 0,
+        _i32(kv_len, s, "kv_len"), pos_at, pos_stride, _i32(q_len, s, "q_len"), _stream_of(stream, dev))
+    return _checked(_launch(_entry("sixi_qk_rope"), packed, dev), check)
 
 
 class DraftVerify(_Workspace):
@@ -1202,23 +1248,33 @@ class DraftVerify(_Workspace):
 
     Keeps a device workspace: calls of one object must be ordered on one stream, as :class:`Kv8Attention`'s."""
 
-    def params(self, logits, draft, u, u_next, keep, token, draft_probs=None, q_len=None, temperature=None) -> SixiDraftParams:
-        import torch
+    _struct = SixiDraftParams
+    _entries = ("sixi_draft_verify", "sixi_draft_workspace_bytes")
 
-        p = SixiDraftParams()
-        s, n = logits.shape[:2]
-        p.logits = _rows_view(logits)
-        if draft_probs is not None and n > 1:
-            p.draft_probs = _rows_view(draft_probs)
+    @staticmethod
+    def _packer(logits, draft, u, u_next, keep, token, draft_probs, q_len, temperature, stream):
+        torch = _torch()
+        view = _rows3(logits, "logits")
+        s, n = view[5], view[4]
+        ids = (0, 0, 0, 0)
+        probs = _NO_VIEW
         if n > 1:
             for t, kind, what in ((draft, torch.int32, "draft: expected int32"), (u, torch.float32, "u: expected float32")):
-                if t is None or t.dtype != kind or t.dim() != 2 or t.shape[0] < s or t.shape[1] < n - 1 or (n > 2 and t.stride(1) != 1):
+                if t is None or t.dtype is not kind or t.dim() != 2 or t.shape[0] < s or t.shape[1] < n - 1 or (
+                        n > 2 and t.stride(1) != 1):
                     raise ValueError(what + " [S, rows - 1], rows contiguous")
-            p.draft, p.draft_stride = draft.data_ptr(), draft.stride(0)
-            p.u, p.u_stride = u.data_ptr(), u.stride(0)
-        p.u_next, p.temperature = _f32(u_next, s, "u_next"), _f32(temperature, s, "temperature")
-        p.q_len, p.keep, p.token = _i32(q_len, s, "q_len"), _i32(keep, s, "keep"), _i32(token, s, "token")
-        return p
+            ids = (draft.data_ptr(), draft.stride(0), u.data_ptr(), u.stride(0))
+            if draft_probs is not None:
+                probs = _rows3(draft_probs, "draft_probs")
+        head = (*view, *probs, *ids, _f32(u_next, s, "u_next"), _f32(temperature, s, "temperature"), _i32(q_len, s, "q_len"),
+                _i32(keep, s, "keep"), _i32(token, s, "token"))
+        return lambda at, nbytes: _DRAFT.pack(*head, at, nbytes, 0, 0, stream)
+
+    def params(self, logits, draft, u, u_next, keep, token, draft_probs=None, q_len=None, temperature=None,
+               stream=0) -> SixiDraftParams:
+        """The call's C struct, without a workspace."""
+        return SixiDraftParams.from_buffer_copy(
+            self._packer(logits, draft, u, u_next, keep, token, draft_probs, q_len, temperature, stream)(0, 0))
 
     def __call__(self, logits, draft, u, u_next, keep, token, draft_probs=None, q_len=None, temperature=None, stream=None,
                  check=True, workspace=None) -> int:
@@ -1227,14 +1283,6 @@ class DraftVerify(_Workspace):
         ``u[S, rows - 1]`` and ``u_next[S]`` f32 in [0, 1); ``q_len[S]`` rows of each stream (1 + drafts);
         ``temperature[S]`` f32, 0 for greedy.  Writes ``keep[S]`` (rows that stay: 1 + tokens kept, what the GDN's
         ``snap`` takes) and ``token[S]`` int32."""
-        dev, st = _on_device((logits, draft, u, u_next, keep, token, draft_probs, q_len, temperature, workspace), stream)
-        if dev != self.device:
-            raise ValueError(f"tensors on {dev}, the handle on {self.device}")
-        p = self.params(logits, draft, u, u_next, keep, token, draft_probs, q_len, temperature)
-        p.stream = st
-        rc = self._give(p, self.lib.sixi_draft_workspace_bytes, workspace)
-        if rc != OK:
-            if check:
-                raise SixiAttnError(rc, strerror(rc))
-            return rc
-        return _launch(self.lib.sixi_draft_verify, p, dev, check)
+        dev = _device_of(logits, draft, u, u_next, keep, token, draft_probs, q_len, temperature, workspace)
+        return self._run(self._packer(logits, draft, u, u_next, keep, token, draft_probs, q_len, temperature,
+                                      _stream_of(stream, dev)), dev, workspace, check)
