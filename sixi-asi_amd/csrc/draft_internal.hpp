@@ -23,6 +23,16 @@ struct DraftDraw {
     int32_t last_w, last_p;
 };
 
+// What a stream's rows come to.
+struct DraftVerdict {
+    double inv_z;   // 1 / the sum of the weights of the row below
+    double inv_t;   // 0: greedy
+    int32_t row;    // the row that the next token is drawn from
+    int32_t d;      // its drafted token (V: none in range); -1 behind the last one
+    float top;      // its largest logit
+    int32_t at;     // the lowest token that has it (greedy streams)
+};
+
 struct DraftArgs {
     const char* logits;
     int64_t l_nb1, l_nb2;  // row, stream
@@ -40,6 +50,7 @@ struct DraftArgs {
     int32_t* token;
     DraftPart* parts;  // [S][n_rows][chunks]
     DraftDraw* draws;  // [S][chunks]
+    DraftVerdict* verdicts;  // [S]
     int32_t V, n_rows, S, chunks;
 };
 

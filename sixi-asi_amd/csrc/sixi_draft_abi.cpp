@@ -95,11 +95,13 @@ int resolve(const sixi_draft_params* p, sixi::DraftArgs* out, size_t* ws) {
     a.S = (int32_t)S;
     a.chunks = (int32_t)((V + sixi::kDraftChunk - 1) / sixi::kDraftChunk);
     const int64_t parts = S * rows * a.chunks * (int64_t)sizeof(sixi::DraftPart);  // < 2^16 * 2^10 * 2^18 * 2^4
-    *ws = (size_t)parts + (size_t)(S * a.chunks) * sizeof(sixi::DraftDraw);
+    const int64_t draws = S * a.chunks * (int64_t)sizeof(sixi::DraftDraw);
+    *ws = (size_t)(parts + draws) + (size_t)S * sizeof(sixi::DraftVerdict);
     *ws = (*ws + 255) / 256 * 256;
     if (*ws == 0) *ws = 256;
     a.parts = static_cast<sixi::DraftPart*>(p->workspace);
     a.draws = reinterpret_cast<sixi::DraftDraw*>(static_cast<char*>(p->workspace) + parts);
+    a.verdicts = reinterpret_cast<sixi::DraftVerdict*>(static_cast<char*>(p->workspace) + parts + draws);
     *out = a;
     return SIXI_OK;
 }
