@@ -9,8 +9,9 @@
 namespace sixi {
 
 constexpr int kDraftChunk = 4096;  // logits of a row that one work-group takes
+constexpr int kDraftMaxRows = 1024;
 
-// A chunk of a row: the largest logit, the lowest token that has it, and the sum of exp((l - max) / T).
+// Some chunks of a row: the largest logit, the lowest token that has it, and the sum of exp((l - max) / T).
 struct DraftPart {
     double sum;
     float top;
@@ -26,7 +27,7 @@ struct DraftDraw {
 // What a stream's rows come to.
 struct DraftVerdict {
     double inv_z;   // 1 / the sum of the weights of the row below
-    double inv_t;   // 0: greedy
+    double c;       // log2(e) / temperature; 0: greedy
     int32_t row;    // the row that the next token is drawn from
     int32_t d;      // its drafted token (V: none in range); -1 behind the last one
     float top;      // its largest logit
@@ -48,10 +49,11 @@ struct DraftArgs {
     const int32_t* q_len;
     int32_t* keep;
     int32_t* token;
-    DraftPart* parts;  // [S][n_rows][chunks]
+    DraftPart* parts;  // [S][n_rows][n_parts]
     DraftDraw* draws;  // [S][chunks]
-    DraftVerdict* verdicts;  // [S]
-    int32_t V, n_rows, S, chunks;
+    int32_t* counts;   // [S]: work-groups that have left their share in draws
+    int32_t V, n_rows, S, chunks;  // chunks of a row
+    int32_t run, n_parts;          // chunks that a work-group of the rows takes; such work-groups of a row
 };
 
 hipError_t launch_draft_verify(const DraftArgs& a, hipStream_t stream);

@@ -1,16 +1,17 @@
 // draft_verify.hip -- which drafted tokens stay, and the token behind them (include/sixi_draft.h).
 //
-// Three launches, each a function of its inputs alone (no atomics on sums, every sum in a fixed order):
+// Two launches, a function of the inputs alone (every sum in a fixed order):
 //   rows    every row's chunks of 4096 logits: largest, its token (where a greedy stream asks for it), sum of
-//           exp((l - max) / T)
+//           2^((l - max) log2(e) / T)
 //   draw    per stream, the accept chain from those sums (a few hundred numbers, formed again by each
-//           work-group), then the chunk's share of the row that the next token is drawn from
-//   find    the chunk and the token at which the running sum passes u_next * total
+//           work-group), then the chunk's share of the row that the next token is drawn from; the stream's
+//           last work-group to get there finds the chunk and the token at which the running sum passes
+//           u_next * total
 // Bound by HBM: the logits once (the row that is drawn from a second time, out of the caches).  Sums and
 // exponentials run in 64 bits: a token is found between neighbours of a running sum over the whole
-// vocabulary, where 1e-7 of the total spans many of them.  exp is formed from its power of two and a
-// polynomial of degree 8 in the rest (Chebyshev interpolation on +-ln(2)/2: off by at most 1.1e-12), about
-// 16 f64 instructions, next to the loads.
+// vocabulary, where 1e-7 of the total spans many of them.  2^x is its whole part, from the sum with 1.5 * 2^52,
+// added to the exponent of a polynomial of degree 8 in the rest (Chebyshev interpolation on +-1/2: off by at
+// most 1.1e-12): 14 f64 instructions, next to the loads.
 #include <hip/hip_runtime.h>
 
 #include "draft_internal.hpp"
@@ -21,26 +22,27 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPer = kDraftChunk / kThreads;  // logits per thread
+constexpr double kLog2e = 1.4426950408889634;
 
-// exp(x) for x <= 0 (0 below -700)
-__device__ __forceinline__ double exp_neg(double x) {
-    const double n = rint(x * 1.4426950408889634);
-    const double r = fma(n, -0.6931471805599453, x);  // (off by 2.4e-17 n: below 3e-14 of the result)
-    double p = 2.4884309742982776e-05;
-    p = fma(p, r, 0.00019915868734151192);
-    p = fma(p, r, 0.0013888802102825077);
-    p = fma(p, r, 0.00833326609438625);
-    p = fma(p, r, 0.041666667037968945);
-    p = fma(p, r, 0.1666666689106594);
-    p = fma(p, r, 0.4999999999944456);
-    p = fma(p, r, 0.9999999999797822);
-    p = fma(p, r, 1.0000000000000133);
-    return x > -700.0 ? ldexp(p, (int)n) : 0.0;
+// The polynomial of 2^x on [-1/2, 1/2], highest power first.
+constexpr double kPoly[9] = {1.3259565309065025e-06, 1.5310080791697267e-05, 0.00015403434142954517, 0.0013333450562298989, 0.009618129193338041,
+                             0.055504109412126475, 0.2402265069564321, 0.6931471805459314, 1.0000000000000133};
+
+// 2^y for y <= 0 (0 below -1000 and for NaN)
+__device__ __forceinline__ double exp2_neg(double y) {
+    constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52: the sum's low bits are y's nearest whole number
+    const double z = fmax(y, -1000.0), t = z + kWhole, r = z - (t - kWhole);
+    double p = kPoly[0];
+#pragma unroll
+    for (int k = 1; k < 9; ++k) p = fma(p, r, kPoly[k]);
+    p = __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+    return y > -1000.0 ? p : 0.0;
 }
 
-// exp((l - top) / T): 1 at the top itself (also where both are infinite), 0 for -inf and NaN
-__device__ __forceinline__ double weight(float l, float top, double inv_t) {
-    return l == top ? 1.0 : exp_neg(((double)l - (double)top) * inv_t);
+// exp((l - top) / T) with c = log2(e) / T; 0 for -inf and NaN.  Where the top is infinite, its equals take all.
+__device__ __forceinline__ double weight(float l, float top, double c) {
+    if (top == __builtin_huge_valf()) return l == top ? 1.0 : 0.0;
+    return exp2_neg(fma((double)l, c, -(double)top * c));
 }
 
 __device__ __forceinline__ float load1(const char* p, int type) {
@@ -98,51 +100,140 @@ __device__ __forceinline__ void load_vec(const char* row, int t, int V, float* x
     }
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, 64));
-    return x;
+// Moves within the 16 lanes of a row (DPP), and reductions and running sums from them: a few cycles a step,
+// where a shuffle through LDS takes a hundred.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x, int none) {
+    return __builtin_amdgcn_update_dpp(none, x, CTRL, 0xf, 0xf, false);
 }
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-    return x;
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x, float none) {
+    return __int_as_float(dpp<CTRL>(__float_as_int(x), __float_as_int(none)));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x, double none) {
+    return __hiloint2double(dpp<CTRL>(__double2hiint(x), __double2hiint(none)), dpp<CTRL>(__double2loint(x), __double2loint(none)));
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140, kShr1 = 0x111;
+__device__ __forceinline__ int lane_of(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
+__device__ __forceinline__ float lane_of(float x, int l) { return __int_as_float(lane_of(__float_as_int(x), l)); }
+__device__ __forceinline__ double lane_of(double x, int l) { return __hiloint2double(lane_of(__double2hiint(x), l), lane_of(__double2loint(x), l)); }
+
+// f over the 16 lanes of a row, then over the wave's four rows; the result in every lane.
+template <typename T, typename F>
+__device__ __forceinline__ T row_reduce(T x, F f) {
+    x = f(x, dpp<kXor1>(x, x));
+    x = f(x, dpp<kXor2>(x, x));
+    x = f(x, dpp<kHalfMirror>(x, x));
+    return f(x, dpp<kMirror>(x, x));
+}
+template <typename T, typename F>
+__device__ __forceinline__ T wave_reduce(T x, F f) {
+    x = row_reduce(x, f);
+    return f(f(lane_of(x, 0), lane_of(x, 16)), f(lane_of(x, 32), lane_of(x, 48)));
+}
+struct Plus {
+    __device__ __forceinline__ double operator()(double a, double b) const { return a + b; }
+};
+struct Greater {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+    __device__ __forceinline__ int operator()(int a, int b) const { return max(a, b); }
+};
+struct Less {
+    __device__ __forceinline__ int operator()(int a, int b) const { return min(a, b); }
+};
+
+// The sum of the lanes in front of one's own, and of all.
+__device__ __forceinline__ double wave_before(double x, double& total) {
+    double run = x;
+    run += dpp<0x111>(run, 0.0);
+    run += dpp<0x112>(run, 0.0);
+    run += dpp<0x114>(run, 0.0);
+    run += dpp<0x118>(run, 0.0);
+    const double r0 = lane_of(run, 15), r1 = lane_of(run, 31), r2 = lane_of(run, 47), r3 = lane_of(run, 63);
+    const int row = (threadIdx.x & 63) >> 4;
+    const double front = row == 0 ? 0.0 : row == 1 ? r0 : row == 2 ? r0 + r1 : (r0 + r1) + r2;
+    total = ((r0 + r1) + r2) + r3;
+    return dpp<kShr1>(run, 0.0) + front;
 }
 
-// A wave takes a quarter of the chunk by itself; the four are joined behind the only barrier.
+// exp2_neg's sum over a thread's logits, for a total only: what is hidden or far below counts 2^-1000.
+__device__ __forceinline__ double sum_of(const float (&x)[kPer], float top, double c, float least) {
+    constexpr double kWhole = 6755399441055744.0;
+    const double off = -(double)top * c;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const double y = fma((double)fmaxf(x[i], least), c, off), t = y + kWhole, r = y - (t - kWhole);
+        double p = kPoly[0];
+#pragma unroll
+        for (int k = 1; k < 9; ++k) p = fma(p, r, kPoly[k]);
+        sum += __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+    }
+    return sum;
+}
+
+// A work-group takes a.run chunks of a row, the next one's loads ahead of the sums over the last; its waves go
+// by themselves, each with a running maximum and a sum relative to it, and are joined behind the only barrier.
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void draft_rows_kernel(DraftArgs a) {
     constexpr int kVec = Elem<TYPE>::per, kWaves = kThreads / 64;
     __shared__ float tops[kWaves];
     __shared__ int ats[kWaves];
     __shared__ double sums[kWaves];
-    const int chunk = blockIdx.x, j = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
+    const int part = blockIdx.x, j = blockIdx.y, s = blockIdx.z, tid = threadIdx.x;
     if (j >= rows_of(a, s)) return;
+    if (part == 0 && j == 0 && tid == 0) a.counts[s] = 0;  // for the next launch
     const char* row = a.logits + (int64_t)j * a.l_nb1 + (int64_t)s * a.l_nb2;
-    float x[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; i += kVec) load_vec<TYPE>(row, chunk * kDraftChunk + i * kThreads + tid * kVec, a.V, x + i);
     const float heat = heat_of(a, s);
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < kPer; ++i) top = fmaxf(top, x[i]);  // (fmaxf passes over NaN)
-    top = wave_max(top);
-    if (!(top > -__builtin_huge_valf())) top = -__builtin_huge_valf();  // (a wave of NaN)
+    const bool hot = heat > 0.0f;
+    const double c = hot ? kLog2e / (double)heat : 0.0;
+    const float span = hot ? (float)(1000.0 / c) : 0.0f;
+    const int first = part * a.run, last = min(first + a.run, a.chunks);
+    const float none = -__builtin_huge_valf();
+    float top = none;
     int at = a.V;
     double sum = 0.0;
-    if (!(heat > 0.0f)) {
+    float next[kPer];
+    auto load = [&](int chunk) {
 #pragma unroll
-        for (int i = kPer - 1; i >= 0; --i)
-            if (x[i] == top) at = min(at, chunk * kDraftChunk + i / kVec * kVec * kThreads + tid * kVec + i % kVec);
-        if (!(top > -__builtin_huge_valf())) at = a.V;
+        for (int i = 0; i < kPer; i += kVec) load_vec<TYPE>(row, chunk * kDraftChunk + i * kThreads + tid * kVec, a.V, next + i);
+    };
+    load(first);
+    for (int chunk = first; chunk < last; ++chunk) {
+        float x[kPer];
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o, 64));
-    } else if (top > -__builtin_huge_valf()) {
-        const double inv_t = 1.0 / (double)heat;
+        for (int i = 0; i < kPer; ++i) x[i] = next[i];
+        if (chunk + 1 < last) load(chunk + 1);
+        float here = x[0];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += weight(x[i], top, inv_t);
-        sum = wave_sum(sum);
+        for (int i = 1; i < kPer; ++i) here = fmaxf(here, x[i]);  // (fmaxf passes over NaN)
+        here = wave_reduce(here, Greater());
+        if (!(here > none)) continue;  // (nothing but -inf and NaN)
+        if (!hot) {
+            if (here > top) {
+                int h = a.V;
+#pragma unroll
+                for (int i = kPer - 1; i >= 0; --i)
+                    if (x[i] == here) h = min(h, chunk * kDraftChunk + i / kVec * kVec * kThreads + tid * kVec + i % kVec);
+                at = wave_reduce(h, Less());
+                top = here;
+            }
+        } else if (here == __builtin_huge_valf()) {  // infinite logits share everything
+            double n = 0.0;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) n += x[i] == here ? 1.0 : 0.0;
+            sum = top == here ? sum + n : n;
+            top = here;
+        } else if (top < __builtin_huge_valf()) {
+            if (here > top) {
+                sum *= weight(top, here, c);
+                top = here;
+            }
+            sum += sum_of(x, top, c, top - span);
+        }
     }
+    sum = wave_reduce(sum, Plus());
     if (tid % 64 == 0) {
         tops[tid / 64] = top;
         ats[tid / 64] = at;
@@ -155,12 +246,11 @@ __global__ __launch_bounds__(kThreads) void draft_rows_kernel(DraftArgs a) {
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) take_top(best, best_at, tops[w], ats[w]);
         double z = 0.0;
-        if (heat > 0.0f && best > -__builtin_huge_valf()) {
-            const double inv_t = 1.0 / (double)heat;
+        if (hot && best > none) {
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) z += sums[w] * weight(tops[w], best, inv_t);
+            for (int w = 0; w < kWaves; ++w) z += sums[w] * weight(tops[w], best, c);
         }
-        DraftPart& p = a.parts[((int64_t)s * a.n_rows + j) * a.chunks + chunk];
+        DraftPart& p = a.parts[((int64_t)s * a.n_rows + j) * a.n_parts + part];
         p.sum = z;
         p.top = best;
         p.at = best_at;
@@ -169,53 +259,62 @@ __global__ __launch_bounds__(kThreads) void draft_rows_kernel(DraftArgs a) {
 
 constexpr int kGroup = 16;  // lanes that sum a row's chunks
 
+struct RowSum {
+    double z;
+    float top;
+    int at;
+};
 // A row's largest logit and sum of weights, by the 16 lanes of a group (every lane gets them).
-__device__ __forceinline__ void row_sum(const DraftArgs& a, int s, int j, double inv_t, float& top, int& at, double& z) {
+__device__ __forceinline__ RowSum row_sum(const DraftArgs& a, int s, int j, double c) {
     const int lane = threadIdx.x % kGroup;
-    const DraftPart* parts = a.parts + ((int64_t)s * a.n_rows + j) * a.chunks;
-    top = -__builtin_huge_valf();
-    at = a.V;
+    const DraftPart* parts = a.parts + ((int64_t)s * a.n_rows + j) * a.n_parts;
+    RowSum r{0.0, -__builtin_huge_valf(), a.V};
 #pragma unroll 4
-    for (int c = lane; c < a.chunks; c += kGroup) take_top(top, at, parts[c].top, parts[c].at);
-#pragma unroll
-    for (int o = kGroup / 2; o > 0; o >>= 1) take_top(top, at, __shfl_xor(top, o, 64), __shfl_xor(at, o, 64));
-    z = 0.0;
+    for (int i = lane; i < a.n_parts; i += kGroup) take_top(r.top, r.at, parts[i].top, parts[i].at);
+    const float mine = r.top;
+    r.top = row_reduce(mine, Greater());
+    r.at = row_reduce(mine == r.top ? r.at : a.V, Less());
 #pragma unroll 4
-    for (int c = lane; c < a.chunks; c += kGroup) z += parts[c].sum * weight(parts[c].top, top, inv_t);
-#pragma unroll
-    for (int o = kGroup / 2; o > 0; o >>= 1) z += __shfl_xor(z, o, 64);
+    for (int i = lane; i < a.n_parts; i += kGroup) r.z += parts[i].sum * weight(parts[i].top, r.top, c);
+    r.z = row_reduce(r.z, Plus());
+    return r;
 }
 
-// Each group of 16 lanes judges rows of its own; `stop` (LDS) is then the first whose token goes, or the
-// last row.  Every thread of the work-group calls this.
-__device__ __forceinline__ DraftVerdict decide(const DraftArgs& a, int s, int rows, int* stop) {
+// Each group of 16 lanes judges rows of its own; `stop` is then the first whose token goes, or the last
+// row.  Every thread of the work-group calls this; `sums` (a row each) and `stop` are in LDS.
+__device__ __forceinline__ DraftVerdict decide(const DraftArgs& a, int s, int rows, RowSum* sums, int* stop) {
     const float heat = heat_of(a, s);
-    const bool greedy = !(heat > 0.0f);
     DraftVerdict v{};
-    v.inv_t = greedy ? 0.0 : 1.0 / (double)heat;
+    v.c = heat > 0.0f ? kLog2e / (double)heat : 0.0;
     if (threadIdx.x == 0) *stop = rows - 1;
     __syncthreads();
-    for (int j = threadIdx.x / kGroup; j < rows - 1; j += kThreads / kGroup) {
-        float top;
-        int at;
-        double z, p = 0.0, q = 1.0;
-        const int d = a.draft[(int64_t)s * a.draft_stride + j];
+    for (int j = threadIdx.x / kGroup; j < rows; j += kThreads / kGroup) {
+        float l = 0.0f, u = 0.0f;
+        double p = 0.0, q = 1.0;
+        int d = -1;
+        if (j < rows - 1) {
+            d = a.draft[(int64_t)s * a.draft_stride + j];
+            u = a.u[(int64_t)s * a.u_stride + j];
+        }
         const bool known = d >= 0 && d < a.V;
-        float l = 0.0f;
         if (known) {
             l = load1(a.logits + (int64_t)j * a.l_nb1 + (int64_t)s * a.l_nb2 + (int64_t)d * bytes_of(a.l_type), a.l_type);
             if (a.probs)
                 q = load1(a.probs + (int64_t)j * a.p_nb1 + (int64_t)s * a.p_nb2 + (int64_t)d * bytes_of(a.p_type), a.p_type);
         }
-        row_sum(a, s, j, v.inv_t, top, at, z);
-        if (known) p = greedy ? (d == at ? 1.0 : 0.0) : z > 0.0 ? weight(l, top, v.inv_t) / z : 0.0;
-        if (!((double)a.u[(int64_t)s * a.u_stride + j] * q < p) && threadIdx.x % kGroup == 0) atomicMin(stop, j);
+        const RowSum r = row_sum(a, s, j, v.c);
+        if (threadIdx.x % kGroup == 0) {
+            sums[j] = r;
+            if (known) p = v.c == 0.0 ? (d == r.at ? 1.0 : 0.0) : r.z > 0.0 ? weight(l, r.top, v.c) / r.z : 0.0;
+            if (j < rows - 1 && !((double)u * q < p)) atomicMin(stop, j);
+        }
     }
     __syncthreads();
     v.row = *stop;
-    double z;
-    row_sum(a, s, v.row, v.inv_t, v.top, v.at, z);
-    v.inv_z = z > 0.0 ? 1.0 / z : 0.0;
+    const RowSum r = sums[v.row];
+    v.top = r.top;
+    v.at = r.at;
+    v.inv_z = r.z > 0.0 ? 1.0 / r.z : 0.0;
     v.d = -1;
     if (v.row < rows - 1) {
         v.d = a.draft[(int64_t)s * a.draft_stride + v.row];
@@ -233,7 +332,7 @@ __device__ __forceinline__ void weights_of(const DraftArgs& a, int s, const Draf
         x[i] = -__builtin_huge_valf();
         q[i] = 0.0f;
     }
-    const bool hot = v.inv_t != 0.0 && v.top > -__builtin_huge_valf();
+    const bool hot = v.c != 0.0 && v.top > -__builtin_huge_valf();
     if (hot) {
         const char* row = a.logits + (int64_t)v.row * a.l_nb1 + (int64_t)s * a.l_nb2;
 #pragma unroll
@@ -254,7 +353,7 @@ __device__ __forceinline__ void weights_of(const DraftArgs& a, int s, const Draf
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int t = t0 + i;
-        p[i] = hot ? weight(x[i], v.top, v.inv_t) * v.inv_z : v.inv_t == 0.0 && t == v.at ? 1.0 : 0.0;
+        p[i] = hot ? weight(x[i], v.top, v.c) * v.inv_z : v.c == 0.0 && t == v.at ? 1.0 : 0.0;
         if (t >= a.V) p[i] = 0.0;
         w[i] = p[i];
         if (v.d >= 0) {
@@ -265,90 +364,35 @@ __device__ __forceinline__ void weights_of(const DraftArgs& a, int s, const Draf
     }
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(kThreads) void draft_draw_kernel(DraftArgs a) {
-    __shared__ double ws[kThreads / 64], ps[kThreads / 64];
-    __shared__ int lws[kThreads / 64], lps[kThreads / 64], stop;
-    const int chunk = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
-    const int rows = rows_of(a, s);
-    if (rows == 0) {
-        if (chunk == 0 && tid == 0) {
-            a.keep[s] = 0;
-            a.token[s] = -1;
-        }
-        return;
-    }
-    const DraftVerdict v = decide(a, s, rows, &stop);
-    if (chunk == 0 && tid == 0) {
-        a.keep[s] = v.row + 1;
-        a.verdicts[s] = v;  // for the last launch
-    }
-    double w[kPer], p[kPer];
-    const int t0 = chunk * kDraftChunk + tid * kPer;
-    weights_of<TYPE>(a, s, v, t0, w, p);
-    double sum_w = 0.0, sum_p = 0.0;
-    int last_w = -1, last_p = -1;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        sum_w += w[i];
-        sum_p += p[i];
-        if (w[i] > 0.0) last_w = t0 + i;
-        if (p[i] > 0.0) last_p = t0 + i;
-    }
-    sum_w = wave_sum(sum_w);
-    sum_p = wave_sum(sum_p);
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        last_w = max(last_w, __shfl_xor(last_w, o, 64));
-        last_p = max(last_p, __shfl_xor(last_p, o, 64));
-    }
-    if (tid % 64 == 0) {
-        ws[tid / 64] = sum_w;
-        ps[tid / 64] = sum_p;
-        lws[tid / 64] = last_w;
-        lps[tid / 64] = last_p;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        DraftDraw& d = a.draws[(int64_t)s * a.chunks + chunk];
-        d.w = ((ws[0] + ws[1]) + ws[2]) + ws[3];
-        d.p = ((ps[0] + ps[1]) + ps[2]) + ps[3];
-        d.last_w = max(max(lws[0], lws[1]), max(lws[2], lws[3]));
-        d.last_p = max(max(lps[0], lps[1]), max(lps[2], lps[3]));
-    }
+// What other work-groups wrote in the same launch: loads and stores at the device's scope, past the caches
+// that are not shared.
+__device__ __forceinline__ void put(DraftDraw* d, const DraftDraw& x) {
+    __hip_atomic_store(&d->w, x.w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&d->p, x.p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&d->last_w, x.last_w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&d->last_p, x.last_p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ DraftDraw get(DraftDraw* d) {
+    return {__hip_atomic_load(&d->w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), __hip_atomic_load(&d->p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+            __hip_atomic_load(&d->last_w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT),
+            __hip_atomic_load(&d->last_p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)};
 }
 
-// The sum of the lanes in front of one's own (a wave's running sum, by doubling steps).
-__device__ __forceinline__ double wave_before(double x, double& total) {
-    const int lane = threadIdx.x & 63;
-    double run = x;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(run, o, 64);
-        if (lane >= o) run += y;
-    }
-    total = __shfl(run, 63, 64);
-    const double y = __shfl_up(run, 1, 64);
-    return lane > 0 ? y : 0.0;
-}
-
+// The token, by one work-group.
 template <int TYPE>
-__global__ __launch_bounds__(kThreads) void draft_find_kernel(DraftArgs a) {
-    __shared__ double sums[kThreads / 64];
-    __shared__ int first;
-    const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-    if (rows_of(a, s) == 0) return;
-    const DraftVerdict v = a.verdicts[s];
-    const DraftDraw* d = a.draws + (int64_t)s * a.chunks;
+__device__ __forceinline__ void find_token(const DraftArgs& a, int s, const DraftVerdict& v, double* sums, int* first) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    DraftDraw* draws = a.draws + (int64_t)s * a.chunks;
     // totals of the draw's weights and of p, then the first chunk whose end is past the mark; where the sums'
     // rounding (or u_next = 1) leaves none, the last one with a weight.  Every wave does this alike.
     double total = 0.0, total_p = 0.0;
     for (int c = lane; c < a.chunks; c += 64) {
-        total += d[c].w;
-        total_p += d[c].p;
+        const DraftDraw d = get(draws + c);
+        total += d.w;
+        total_p += d.p;
     }
-    total = wave_sum(total);
-    total_p = wave_sum(total_p);
+    total = wave_reduce(total, Plus());
+    total_p = wave_reduce(total_p, Plus());
     const bool from_w = total > 0.0;
     if (!from_w) total = total_p;
     if (!(total > 0.0)) {
@@ -359,18 +403,18 @@ __global__ __launch_bounds__(kThreads) void draft_find_kernel(DraftArgs a) {
     double before = 0.0, ahead = 0.0;
     int chunk = 0, last = -1;
     for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-        const int c = c0 + lane;
-        const bool in = c < a.chunks;
-        const double mine = in ? (from_w ? d[c].w : d[c].p) : 0.0;
-        const int tail = in ? (from_w ? d[c].last_w : d[c].last_p) : -1;
+        const DraftDraw d = get(draws + min(c0 + lane, a.chunks - 1));
+        const bool in = c0 + lane < a.chunks;
+        const double mine = in ? (from_w ? d.w : d.p) : 0.0;
+        const int tail = in ? (from_w ? d.last_w : d.last_p) : -1;
         double sum;
         const double at = ahead + wave_before(mine, sum);
         const uint64_t some = __builtin_amdgcn_ballot_w64(tail >= 0), past = __builtin_amdgcn_ballot_w64(tail >= 0 && at + mine > mark);
         if (some) {
             const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
             chunk = c0 + l;
-            before = __shfl(at, l, 64);
-            last = __shfl(tail, l, 64);
+            before = lane_of(at, l);
+            last = lane_of(tail, l);
         }
         if (past) break;
         ahead += sum;
@@ -384,16 +428,16 @@ __global__ __launch_bounds__(kThreads) void draft_find_kernel(DraftArgs a) {
     for (int i = 0; i < kPer; ++i) mine += from_w ? w[i] : p[i];
     double at = wave_before(mine, sum);
     if (lane == 63) sums[tid / 64] = sum;
-    if (tid == 0) first = kThreads;
+    if (tid == 0) *first = kThreads;
     __syncthreads();
     double front = before;
     for (int k = 0; k < tid / 64; ++k) front += sums[k];
     at += front;
-    if (mine > 0.0 && at + mine > mark) atomicMin(&first, tid);
+    if (mine > 0.0 && at + mine > mark) atomicMin(first, tid);
     __syncthreads();
-    if (first == kThreads) {  // (the chunk's end is past the mark by less than its sums' rounding)
+    if (*first == kThreads) {  // (the chunk's end is past the mark by less than its sums' rounding)
         if (tid == 0) a.token[s] = last;
-    } else if (tid == first) {
+    } else if (tid == *first) {
         int found = -1;
         bool done = false;
 #pragma unroll
@@ -410,14 +454,62 @@ __global__ __launch_bounds__(kThreads) void draft_find_kernel(DraftArgs a) {
 }
 
 template <int TYPE>
+__global__ __launch_bounds__(kThreads) void draft_draw_kernel(DraftArgs a) {
+    __shared__ double ws[kThreads / 64], ps[kThreads / 64];
+    __shared__ int lws[kThreads / 64], lps[kThreads / 64], stop, last;
+    __shared__ RowSum sums[kDraftMaxRows];
+    const int chunk = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const int rows = rows_of(a, s);
+    if (rows == 0) {
+        if (chunk == 0 && tid == 0) {
+            a.keep[s] = 0;
+            a.token[s] = -1;
+        }
+        return;
+    }
+    const DraftVerdict v = decide(a, s, rows, sums, &stop);
+    if (chunk == 0 && tid == 0) a.keep[s] = v.row + 1;
+    double w[kPer], p[kPer];
+    const int t0 = chunk * kDraftChunk + tid * kPer;
+    weights_of<TYPE>(a, s, v, t0, w, p);
+    double sum_w = 0.0, sum_p = 0.0;
+    int last_w = -1, last_p = -1;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        sum_w += w[i];
+        sum_p += p[i];
+        if (w[i] > 0.0) last_w = t0 + i;
+        if (p[i] > 0.0) last_p = t0 + i;
+    }
+    sum_w = wave_reduce(sum_w, Plus());
+    sum_p = wave_reduce(sum_p, Plus());
+    last_w = wave_reduce(last_w, Greater());
+    last_p = wave_reduce(last_p, Greater());
+    if (tid % 64 == 0) {
+        ws[tid / 64] = sum_w;
+        ps[tid / 64] = sum_p;
+        lws[tid / 64] = last_w;
+        lps[tid / 64] = last_p;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        put(a.draws + (int64_t)s * a.chunks + chunk,
+            {((ws[0] + ws[1]) + ws[2]) + ws[3], ((ps[0] + ps[1]) + ps[2]) + ps[3], max(max(lws[0], lws[1]), max(lws[2], lws[3])),
+             max(max(lps[0], lps[1]), max(lps[2], lps[3]))});
+        // counted once the stores above have reached the device's memory
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        last = __hip_atomic_fetch_add(a.counts + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+    }
+    __syncthreads();
+    if (last) find_token<TYPE>(a, s, v, ws, &stop);
+}
+
+template <int TYPE>
 hipError_t launch(const DraftArgs& a, hipStream_t stream) {
-    hipLaunchKernelGGL(draft_rows_kernel<TYPE>, dim3((unsigned)a.chunks, (unsigned)a.n_rows, (unsigned)a.S), dim3(kThreads), 0, stream, a);
-    hipError_t e = hipGetLastError();
+    hipLaunchKernelGGL(draft_rows_kernel<TYPE>, dim3((unsigned)a.n_parts, (unsigned)a.n_rows, (unsigned)a.S), dim3(kThreads), 0, stream, a);
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(draft_draw_kernel<TYPE>, dim3((unsigned)a.chunks, (unsigned)a.S), dim3(kThreads), 0, stream, a);
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(draft_find_kernel<TYPE>, dim3((unsigned)a.S), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 

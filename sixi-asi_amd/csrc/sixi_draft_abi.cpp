@@ -8,6 +8,7 @@
 #include <cstdint>
 
 #include "abi_util.hpp"
+#include "device_util.hpp"
 #include "draft_internal.hpp"
 #include "sixi_draft.h"
 
@@ -15,7 +16,7 @@ namespace {
 
 using namespace sixi_abi;
 
-constexpr int64_t kMaxRows = 1024, kMaxDraftStreams = 65535, kMaxVocab = (int64_t)1 << 30;
+constexpr int64_t kMaxRows = sixi::kDraftMaxRows, kMaxDraftStreams = 65535, kMaxVocab = (int64_t)1 << 30;
 
 int type_bytes(int32_t t) { return t == SIXI_TYPE_F32 ? 4 : t == SIXI_TYPE_F16 || t == SIXI_TYPE_BF16 ? 2 : 0; }
 
@@ -94,14 +95,17 @@ int resolve(const sixi_draft_params* p, sixi::DraftArgs* out, size_t* ws) {
     a.n_rows = (int32_t)rows;
     a.S = (int32_t)S;
     a.chunks = (int32_t)((V + sixi::kDraftChunk - 1) / sixi::kDraftChunk);
-    const int64_t parts = S * rows * a.chunks * (int64_t)sizeof(sixi::DraftPart);  // < 2^16 * 2^10 * 2^18 * 2^4
+    // four chunks in a row where one each would be more than four work-groups for each of 8 places of a CU
+    a.run = S * rows * a.chunks > 4 * 8 * (int64_t)sixi::device_cu_count() ? 4 : 1;
+    a.n_parts = (a.chunks + a.run - 1) / a.run;
+    const int64_t parts = S * rows * a.n_parts * (int64_t)sizeof(sixi::DraftPart);  // < 2^16 * 2^10 * 2^18 * 2^4
     const int64_t draws = S * a.chunks * (int64_t)sizeof(sixi::DraftDraw);
-    *ws = (size_t)(parts + draws) + (size_t)S * sizeof(sixi::DraftVerdict);
+    *ws = (size_t)(parts + draws) + (size_t)S * sizeof(int32_t);
     *ws = (*ws + 255) / 256 * 256;
     if (*ws == 0) *ws = 256;
     a.parts = static_cast<sixi::DraftPart*>(p->workspace);
     a.draws = reinterpret_cast<sixi::DraftDraw*>(static_cast<char*>(p->workspace) + parts);
-    a.verdicts = reinterpret_cast<sixi::DraftVerdict*>(static_cast<char*>(p->workspace) + parts + draws);
+    a.counts = reinterpret_cast<int32_t*>(static_cast<char*>(p->workspace) + parts + draws);
     *out = a;
     return SIXI_OK;
 }
