@@ -263,18 +263,19 @@ struct RowSum {
     double z;
     float top;
     int at;
+    int d;  // the row's drafted token, -1 for none
 };
 // A row's largest logit and sum of weights, by the 16 lanes of a group (every lane gets them).
 __device__ __forceinline__ RowSum row_sum(const DraftArgs& a, int s, int j, double c) {
     const int lane = threadIdx.x % kGroup;
     const DraftPart* parts = a.parts + ((int64_t)s * a.n_rows + j) * a.n_parts;
-    RowSum r{0.0, -__builtin_huge_valf(), a.V};
+    RowSum r{0.0, -__builtin_huge_valf(), a.V, -1};
 #pragma unroll 4
     for (int i = lane; i < a.n_parts; i += kGroup) take_top(r.top, r.at, parts[i].top, parts[i].at);
     const float mine = r.top;
     r.top = row_reduce(mine, Greater());
     r.at = row_reduce(mine == r.top ? r.at : a.V, Less());
-#pragma unroll 4
+#pragma unroll 2
     for (int i = lane; i < a.n_parts; i += kGroup) r.z += parts[i].sum * weight(parts[i].top, r.top, c);
     r.z = row_reduce(r.z, Plus());
     return r;
@@ -302,7 +303,8 @@ __device__ __forceinline__ DraftVerdict decide(const DraftArgs& a, int s, int ro
             if (a.probs)
                 q = load1(a.probs + (int64_t)j * a.p_nb1 + (int64_t)s * a.p_nb2 + (int64_t)d * bytes_of(a.p_type), a.p_type);
         }
-        const RowSum r = row_sum(a, s, j, v.c);
+        RowSum r = row_sum(a, s, j, v.c);
+        r.d = d;
         if (threadIdx.x % kGroup == 0) {
             sums[j] = r;
             if (known) p = v.c == 0.0 ? (d == r.at ? 1.0 : 0.0) : r.z > 0.0 ? weight(l, r.top, v.c) / r.z : 0.0;
@@ -316,10 +318,7 @@ __device__ __forceinline__ DraftVerdict decide(const DraftArgs& a, int s, int ro
     v.at = r.at;
     v.inv_z = r.z > 0.0 ? 1.0 / r.z : 0.0;
     v.d = -1;
-    if (v.row < rows - 1) {
-        v.d = a.draft[(int64_t)s * a.draft_stride + v.row];
-        if (v.d < 0 || v.d > a.V) v.d = a.V;
-    }
+    if (v.row < rows - 1) v.d = r.d >= 0 && r.d < a.V ? r.d : a.V;
     return v;
 }
 
@@ -344,10 +343,12 @@ __device__ __forceinline__ void weights_of(const DraftArgs& a, int s, const Draf
         if (a.p_type == SIXI_TYPE_F32) {
 #pragma unroll
             for (int i = 0; i < kPer; i += 4) load_vec<SIXI_TYPE_F32>(row, t0 + i, a.V, q + i);
+        } else if (a.p_type == SIXI_TYPE_F16) {
+#pragma unroll
+            for (int i = 0; i < kPer; i += 8) load_vec<SIXI_TYPE_F16>(row, t0 + i, a.V, q + i);
         } else {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i)
-                if (t0 + i < a.V) q[i] = load1(row + (int64_t)(t0 + i) * 2, a.p_type);
+            for (int i = 0; i < kPer; i += 8) load_vec<SIXI_TYPE_BF16>(row, t0 + i, a.V, q + i);
         }
     }
 #pragma unroll
@@ -378,130 +379,145 @@ __device__ __forceinline__ DraftDraw get(DraftDraw* d) {
             __hip_atomic_load(&d->last_p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)};
 }
 
-// The token, by one work-group.
-template <int TYPE>
-__device__ __forceinline__ void find_token(const DraftArgs& a, int s, const DraftVerdict& v, double* sums, int* first) {
-    const int tid = threadIdx.x, lane = tid & 63;
+// Where the running sum passes the mark: the chunk, the sum in front of it, its last token with a weight.
+struct DraftFound {
+    double mark, before;
+    int chunk, last;  // chunk -1: no weight at all
+    bool from_w;
+};
+// The first chunk whose end is past the mark; where the sums' rounding (or u_next = 1) leaves none, the last one
+// with a weight.  Every wave does this alike.
+__device__ __forceinline__ DraftFound find_chunk(const DraftArgs& a, int s, double u_next) {
+    const int lane = threadIdx.x & 63;
     DraftDraw* draws = a.draws + (int64_t)s * a.chunks;
-    // totals of the draw's weights and of p, then the first chunk whose end is past the mark; where the sums'
-    // rounding (or u_next = 1) leaves none, the last one with a weight.  Every wave does this alike.
-    double total = 0.0, total_p = 0.0;
-    for (int c = lane; c < a.chunks; c += 64) {
+    const DraftDraw none{0.0, 0.0, -1, -1};
+    const DraftDraw mine0 = lane < a.chunks ? get(draws + lane) : none;  // (most vocabularies: all there is)
+    double total = mine0.w, total_p = mine0.p;
+    for (int c = lane + 64; c < a.chunks; c += 64) {
         const DraftDraw d = get(draws + c);
         total += d.w;
         total_p += d.p;
     }
     total = wave_reduce(total, Plus());
     total_p = wave_reduce(total_p, Plus());
-    const bool from_w = total > 0.0;
-    if (!from_w) total = total_p;
-    if (!(total > 0.0)) {
-        if (tid == 0) a.token[s] = -1;
-        return;
-    }
-    const double mark = (double)a.u_next[s] * total;
-    double before = 0.0, ahead = 0.0;
-    int chunk = 0, last = -1;
+    DraftFound f{0.0, 0.0, -1, -1, total > 0.0};
+    if (!f.from_w) total = total_p;
+    if (!(total > 0.0)) return f;
+    f.mark = u_next * total;
+    double ahead = 0.0;
     for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-        const DraftDraw d = get(draws + min(c0 + lane, a.chunks - 1));
-        const bool in = c0 + lane < a.chunks;
-        const double mine = in ? (from_w ? d.w : d.p) : 0.0;
-        const int tail = in ? (from_w ? d.last_w : d.last_p) : -1;
+        const DraftDraw d = c0 == 0 ? mine0 : c0 + lane < a.chunks ? get(draws + c0 + lane) : none;
+        const double mine = f.from_w ? d.w : d.p;
+        const int tail = f.from_w ? d.last_w : d.last_p;
         double sum;
         const double at = ahead + wave_before(mine, sum);
-        const uint64_t some = __builtin_amdgcn_ballot_w64(tail >= 0), past = __builtin_amdgcn_ballot_w64(tail >= 0 && at + mine > mark);
+        const uint64_t some = __builtin_amdgcn_ballot_w64(tail >= 0), past = __builtin_amdgcn_ballot_w64(tail >= 0 && at + mine > f.mark);
         if (some) {
             const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
-            chunk = c0 + l;
-            before = lane_of(at, l);
-            last = lane_of(tail, l);
+            f.chunk = c0 + l;
+            f.before = lane_of(at, l);
+            f.last = lane_of(tail, l);
         }
         if (past) break;
         ahead += sum;
     }
-    // 16 consecutive tokens per thread, and the running sum over the threads
-    const int t0 = chunk * kDraftChunk + tid * kPer;
-    double w[kPer], p[kPer];
-    weights_of<TYPE>(a, s, v, t0, w, p);
-    double mine = 0.0, sum;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) mine += from_w ? w[i] : p[i];
-    double at = wave_before(mine, sum);
-    if (lane == 63) sums[tid / 64] = sum;
-    if (tid == 0) *first = kThreads;
-    __syncthreads();
-    double front = before;
-    for (int k = 0; k < tid / 64; ++k) front += sums[k];
-    at += front;
-    if (mine > 0.0 && at + mine > mark) atomicMin(first, tid);
-    __syncthreads();
-    if (*first == kThreads) {  // (the chunk's end is past the mark by less than its sums' rounding)
-        if (tid == 0) a.token[s] = last;
-    } else if (tid == *first) {
-        int found = -1;
-        bool done = false;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const double x = from_w ? w[i] : p[i];
-            if (!done && x > 0.0) {
-                at += x;
-                found = t0 + i;
-                done = at > mark;
-            }
-        }
-        a.token[s] = found;
-    }
+    return f;
 }
 
+// A stream's chunks; the last work-group goes through the chunk found once more.
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void draft_draw_kernel(DraftArgs a) {
     __shared__ double ws[kThreads / 64], ps[kThreads / 64];
     __shared__ int lws[kThreads / 64], lps[kThreads / 64], stop, last;
     __shared__ RowSum sums[kDraftMaxRows];
-    const int chunk = blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const int s = blockIdx.y, tid = threadIdx.x;
     const int rows = rows_of(a, s);
     if (rows == 0) {
-        if (chunk == 0 && tid == 0) {
+        if (blockIdx.x == 0 && tid == 0) {
             a.keep[s] = 0;
             a.token[s] = -1;
         }
         return;
     }
+    const double u_next = (double)a.u_next[s];
     const DraftVerdict v = decide(a, s, rows, sums, &stop);
-    if (chunk == 0 && tid == 0) a.keep[s] = v.row + 1;
-    double w[kPer], p[kPer];
-    const int t0 = chunk * kDraftChunk + tid * kPer;
-    weights_of<TYPE>(a, s, v, t0, w, p);
-    double sum_w = 0.0, sum_p = 0.0;
-    int last_w = -1, last_p = -1;
+    if (blockIdx.x == 0 && tid == 0) a.keep[s] = v.row + 1;
+    DraftFound f{0.0, 0.0, (int)blockIdx.x, -1, true};
+#pragma unroll 1
+    for (int pass = 0;; ++pass) {
+        // 16 consecutive tokens per thread
+        double w[kPer], p[kPer];
+        const int t0 = f.chunk * kDraftChunk + tid * kPer;
+        weights_of<TYPE>(a, s, v, t0, w, p);
+        if (pass == 0) {
+            double sum_w = 0.0, sum_p = 0.0;
+            int last_w = -1, last_p = -1;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        sum_w += w[i];
-        sum_p += p[i];
-        if (w[i] > 0.0) last_w = t0 + i;
-        if (p[i] > 0.0) last_p = t0 + i;
+            for (int i = 0; i < kPer; ++i) {
+                sum_w += w[i];
+                sum_p += p[i];
+                if (w[i] > 0.0) last_w = t0 + i;
+                if (p[i] > 0.0) last_p = t0 + i;
+            }
+            sum_w = wave_reduce(sum_w, Plus());
+            sum_p = wave_reduce(sum_p, Plus());
+            last_w = wave_reduce(last_w, Greater());
+            last_p = wave_reduce(last_p, Greater());
+            if (tid % 64 == 0) {
+                ws[tid / 64] = sum_w;
+                ps[tid / 64] = sum_p;
+                lws[tid / 64] = last_w;
+                lps[tid / 64] = last_p;
+            }
+            __syncthreads();
+            if (tid == 0) {
+                put(a.draws + (int64_t)s * a.chunks + f.chunk,
+                    {((ws[0] + ws[1]) + ws[2]) + ws[3], ((ps[0] + ps[1]) + ps[2]) + ps[3], max(max(lws[0], lws[1]), max(lws[2], lws[3])),
+                     max(max(lps[0], lps[1]), max(lps[2], lps[3]))});
+                // counted once the stores above have reached the device's memory
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                last = __hip_atomic_fetch_add(a.counts + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+            }
+            __syncthreads();
+            if (!last) return;
+            f = find_chunk(a, s, u_next);
+            if (f.chunk < 0) {
+                if (tid == 0) a.token[s] = -1;
+                return;
+            }
+            continue;
+        }
+        // the running sum over the threads, then over the tokens of the thread that passes the mark
+        double mine = 0.0, sum;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) mine += f.from_w ? w[i] : p[i];
+        double at = wave_before(mine, sum);
+        if (tid % 64 == 63) ws[tid / 64] = sum;
+        if (tid == 0) stop = kThreads;
+        __syncthreads();
+        double front = f.before;
+        for (int k = 0; k < tid / 64; ++k) front += ws[k];
+        at += front;
+        if (mine > 0.0 && at + mine > f.mark) atomicMin(&stop, tid);
+        __syncthreads();
+        if (stop == kThreads) {  // (the chunk's end is past the mark by less than its sums' rounding)
+            if (tid == 0) a.token[s] = f.last;
+        } else if (tid == stop) {
+            int found = -1;
+            bool done = false;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const double x = f.from_w ? w[i] : p[i];
+                if (!done && x > 0.0) {
+                    at += x;
+                    found = t0 + i;
+                    done = at > f.mark;
+                }
+            }
+            a.token[s] = found;
+        }
+        return;
     }
-    sum_w = wave_reduce(sum_w, Plus());
-    sum_p = wave_reduce(sum_p, Plus());
-    last_w = wave_reduce(last_w, Greater());
-    last_p = wave_reduce(last_p, Greater());
-    if (tid % 64 == 0) {
-        ws[tid / 64] = sum_w;
-        ps[tid / 64] = sum_p;
-        lws[tid / 64] = last_w;
-        lps[tid / 64] = last_p;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        put(a.draws + (int64_t)s * a.chunks + chunk,
-            {((ws[0] + ws[1]) + ws[2]) + ws[3], ((ps[0] + ps[1]) + ps[2]) + ps[3], max(max(lws[0], lws[1]), max(lws[2], lws[3])),
-             max(max(lps[0], lps[1]), max(lps[2], lps[3]))});
-        // counted once the stores above have reached the device's memory
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        last = __hip_atomic_fetch_add(a.counts + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
-    }
-    __syncthreads();
-    if (last) find_token<TYPE>(a, s, v, ws, &stop);
 }
 
 template <int TYPE>
