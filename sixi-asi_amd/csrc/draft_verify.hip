@@ -312,13 +312,16 @@ __device__ __forceinline__ DraftVerdict decide(const DraftArgs& a, int s, int ro
         }
     }
     __syncthreads();
-    v.row = *stop;
+    // (the same in all lanes, and known to be: scalar registers and branches from here on)
+    v.row = lane_of(*stop, 0);
     const RowSum r = sums[v.row];
-    v.top = r.top;
-    v.at = r.at;
-    v.inv_z = r.z > 0.0 ? 1.0 / r.z : 0.0;
+    const int d = lane_of(r.d, 0);
+    const double z = lane_of(r.z, 0);
+    v.top = lane_of(r.top, 0);
+    v.at = lane_of(r.at, 0);
+    v.inv_z = z > 0.0 ? 1.0 / z : 0.0;
     v.d = -1;
-    if (v.row < rows - 1) v.d = r.d >= 0 && r.d < a.V ? r.d : a.V;
+    if (v.row < rows - 1) v.d = d >= 0 && d < a.V ? d : a.V;
     return v;
 }
 
@@ -351,17 +354,24 @@ __device__ __forceinline__ void weights_of(const DraftArgs& a, int s, const Draf
             for (int i = 0; i < kPer; i += 8) load_vec<SIXI_TYPE_BF16>(row, t0 + i, a.V, q + i);
         }
     }
+    // (no branch between the tokens: their polynomials run next to one another)
+    const bool all = v.top == __builtin_huge_valf();
+    const double off = all ? 0.0 : -(double)v.top * v.c;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        const int t = t0 + i;
-        p[i] = hot ? weight(x[i], v.top, v.c) * v.inv_z : v.c == 0.0 && t == v.at ? 1.0 : 0.0;
-        if (t >= a.V) p[i] = 0.0;
-        w[i] = p[i];
-        if (v.d >= 0) {
-            const double less = minus ? p[i] - (double)q[i] : t == v.d ? p[i] - 1.0 : p[i];
-            w[i] = less > 0.0 ? less : 0.0;
-            if (t >= a.V) w[i] = 0.0;
-        }
+        double y = fma((double)x[i], v.c, off);
+        if (all) y = x[i] == v.top ? 0.0 : -2000.0;
+        p[i] = exp2_neg(y) * v.inv_z;  // (0 past the end: -inf there)
+    }
+    if (!hot) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) p[i] = v.c == 0.0 && t0 + i == v.at ? 1.0 : 0.0;
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const double less = minus ? p[i] - (double)fmaxf(q[i], 0.0f) :  // (-inf past the end)
+                                     t0 + i == v.d ? p[i] - 1.0 : p[i];
+        w[i] = v.d < 0 ? p[i] : fmax(less, 0.0);
     }
 }
 
