@@ -112,21 +112,29 @@ struct Cut {
     __device__ __forceinline__ void begin(const Kv8AttnArgs& a) {
         const int lane = threadIdx.x & 63;
         int t = 0, blocks = 0, all = 0, work = 0;
+        // a stream's share of a work-group's blocks, in 1/64 (f32, and then whole numbers: the same sum in
+        // every work-group; kept in range for sums of 512)
+        const float unit = 64.0f * (float)a.Hkv / (float)a.target;
         for (int s0 = 0; s0 < a.S; s0 += 64) {
             stream(a, s0 + lane, t, blocks);
-            // (a stream's share of a work-group's blocks, in 1/64: 2^21 blocks of 2^15 tiles stay in range)
             all += __builtin_amdgcn_readlane(wave_scan(t), 63);
-            work += __builtin_amdgcn_readlane(wave_scan((int)min((int64_t)t * blocks * a.Hkv * 64 / a.target + 1, (int64_t)1 << 22)), 63);
+            work += __builtin_amdgcn_readlane(wave_scan((int)fminf((float)t * (float)blocks * unit, 4194303.0f) + 1), 63);
         }
-        c = (int64_t)all * a.Hkv * 4 >= (int64_t)a.target * 3 ? 1 << 26 : (max((work + 63) / 64, a.least) + 1) / 2 * 2;  // (even: two blocks a step, and of one page)
-        total = 0;
-        if (a.S <= 64)
-            count(a, t, blocks, 0);
-        else
-            for (int s0 = 0; s0 < a.S; s0 += 64) {
-                stream(a, s0 + lane, t, blocks);
-                count(a, t, blocks, total);
-            }
+        // even: two blocks a step, and of one page
+        c = (float)all * (float)a.Hkv >= 0.75f * (float)a.target ? 1 << 26 : (max((work + 63) / 64, a.least) + 1) / 2 * 2;
+        // every stream's last piece is a part of one: longer pieces until they fit the places there are
+        for (int tries = 0;; ++tries) {
+            total = 0;
+            if (a.S <= 64)
+                count(a, t, blocks, 0);
+            else
+                for (int s0 = 0; s0 < a.S; s0 += 64) {
+                    stream(a, s0 + lane, t, blocks);
+                    count(a, t, blocks, total);
+                }
+            if (total <= a.target || c >= 1 << 26 || tries == 3) return;
+            c = (int)((float)c * fminf((float)total / (float)a.target, 1.5f)) / 2 * 2 + 2;
+        }
     }
     // The stream that holds piece `id`, or (by_stream) the place of stream `id`.
     __device__ __forceinline__ Place find(const Kv8AttnArgs& a, int id, bool by_stream) {
@@ -301,24 +309,6 @@ struct Rows {
                 store4(a, row, c * 32 + 2 * i + 4 * h, kv8_f32x4{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]} * inv);
     }
 
-    // Another wave's sums of the same rows, as leave() wrote them.
-    __device__ __forceinline__ void join(const float* part) {
-        const int lane = threadIdx.x & 63, n = lane & 31;
-        if (!live) return;
-        const float m2 = part[32 * D + n], l2 = part[32 * D + 32 + n], up = fmaxf(m, m2);
-        const float f = __builtin_amdgcn_exp2f(m - up), f2 = __builtin_amdgcn_exp2f(m2 - up);
-        m = up;
-        l = l * f + l2 * f2;
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const kv8_f32x4 x = *reinterpret_cast<const kv8_f32x4*>(part + ((c * 4 + i / 4) * 64 + lane) * 4);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[c][i + e] = o[c][i + e] * f + x[e] * f2;
-            }
-    }
-
     __device__ __forceinline__ void leave(float* part) {
         const int lane = threadIdx.x & 63;
         if (!live) return;
@@ -370,24 +360,32 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Work w;
     if (!work_of(a, w)) return;
-    Rows<D> r;
-    r.begin(a, w.n, w.s, w.g, w.tile * 32);
-    const char* mask = MASK ? a.mask + (int64_t)r.j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
-    const int last = min(w.last, (r.reach + kBlk - 1) / kBlk);
+    // cells that any row sees
+    int last = w.last;
+    if (a.mode == SIXI_MASK_BLOCK_CAUSAL)
+        last = min(last, (w.n.cached + (min(w.tile * 32 + 32, w.n.rows * a.G) - 1) / a.G + kBlk) / kBlk);
     const uint32_t k_off = h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
     const uint32_t v_off = n * kBlk + h * 16;
 
-    // K of the next block is asked for when this one's is f16, V when this one's is spent
+    // the first block's codes are asked for before the queries; from then on K of the next block when this
+    // one's is f16, V when this one's is spent
     int b = w.first + wave;
+    kv8_u32x4 kc[KC], vc[KC];
+    int ek = 0, ev = 0;
+    BlockWalk walk;
     if (b < last) {
-        kv8_u32x4 kc[KC], vc[KC];
-        BlockWalk walk;
         walk.begin(a.pages, a.k, a.v, w.s, w.g, b, last);
 #pragma unroll
         for (int c = 0; c < KC; ++c) kc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.k + k_off + c * (kBlk * 32));
-        int ek = *walk.ke, ev = *walk.ve;
+        ek = *walk.ke;
+        ev = *walk.ve;
 #pragma unroll
         for (int c = 0; c < KC; ++c) vc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.v + v_off + c * (kBlk * 32));
+    }
+    Rows<D> r;
+    r.begin(a, w.n, w.s, w.g, w.tile * 32);
+    const char* mask = MASK ? a.mask + (int64_t)r.j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
+    if (b < last) {
         walk.go(a.pages, a.k, a.v, w.s, w.g, kWaves);
         for (; b < last; b += kWaves) {
             f32x16 sc = {};
@@ -423,19 +421,39 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
     }
     r.l = sum_halves(r.l);
 
-    // the waves' results into the first one's, two and then one at a time
-    for (int half = kWaves / 2; half > 0; half /= 2) {
-        float* buf = lds + (wave % half) * tile_floats(D);
-        if (wave >= half && wave < 2 * half) r.leave(buf);
-        __syncthreads();
-        if (wave < half) r.join(buf);
-        __syncthreads();
+    // the waves' results into LDS, and a quarter of the accumulators out of it for each wave
+    r.leave(lds + wave * tile_floats(D));
+    __syncthreads();
+    if (!r.live) return;
+    float m = kLowest, l = 0.0f, f[kWaves];
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        f[k] = lds[k * tile_floats(D) + 32 * D + n];
+        m = fmaxf(m, f[k]);
     }
-    if (wave != 0) return;
-    if (w.pieces == 1)
-        r.finish(a, w.s);
-    else
-        r.leave(a.part + w.id * tile_floats(D));
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) {
+        f[k] = __builtin_amdgcn_exp2f(f[k] - m);
+        l = fmaf(lds[k * tile_floats(D) + 32 * D + 32 + n], f[k], l);
+    }
+    const float inv = w.pieces > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+    char* row = a.out + (int64_t)r.head * a.o_nb1 + (int64_t)r.j * a.o_nb2 + (int64_t)w.s * a.o_nb3;
+    float* part = a.part + w.id * tile_floats(D);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+        const int quad = wave * (D / 32) + i;
+        kv8_f32x4 x = {};
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) x += *reinterpret_cast<const kv8_f32x4*>(lds + k * tile_floats(D) + (quad * 64 + lane) * 4) * f[k];
+        if (w.pieces > 1)
+            *reinterpret_cast<kv8_f32x4*>(part + (quad * 64 + lane) * 4) = x;
+        else
+            store4(a, row, quad / 4 * 32 + quad % 4 * 8 + 4 * h, x * inv);
+    }
+    if (w.pieces > 1 && wave == 0 && h == 0) {
+        part[32 * D + n] = m;
+        part[32 * D + 32 + n] = l;
+    }
 }
 
 // Four waves of 32 rows each over the same cells, NB blocks of 32 a step.  A wave without rows still converts
@@ -599,11 +617,11 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a) {
     const int64_t step = (int64_t)a.Hkv * a.waves * tile_floats(D);  // from piece to piece
     const float* at = a.part + (((int64_t)p.at + (int64_t)(p.tiles - 1 - t32 / a.waves) * p.pieces * a.Hkv + g) * a.waves + t32 % a.waves) * tile_floats(D);
     float m = kLowest;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < p.pieces; ++i) m = fmaxf(m, at[i * step + 32 * D + n]);
     float l = 0.0f;
     kv8_f32x4 o = {};
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < p.pieces; ++i) {
         const float f = __builtin_amdgcn_exp2f(at[i * step + 32 * D + n] - m);
         l = fmaf(at[i * step + 32 * D + 32 + n], f, l);
@@ -617,7 +635,7 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a) {
 template <int D, bool MASK>
 void launch_pieces(const Kv8AttnArgs& a, hipStream_t stream) {
     if (a.waves == 1) {
-        const size_t lds = (size_t)(kWaves / 2) * tile_floats(D) * sizeof(float);
+        const size_t lds = (size_t)kWaves * tile_floats(D) * sizeof(float);
         hipLaunchKernelGGL((kv8_attn_few_kernel<D, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
     } else {
         constexpr int NB = D == 128 ? 2 : 1;
@@ -645,7 +663,7 @@ size_t kv8_attn_plan(Kv8AttnArgs& a) {
     const int64_t t32 = ((int64_t)a.n_q * a.G + 31) / 32;
     a.waves = t32 == 1 ? 1 : kWaves;
     a.target = 2 * device_cu_count();
-    a.least = a.waves == 1 ? 8 : 4;
+    a.least = 4;
     const int64_t tiles = (t32 + a.waves - 1) / a.waves * a.Hkv * a.S;
     const int64_t blocks = (a.n_kv + kBlk - 1) / kBlk;
     // pieces at most: one for each tile, and those that a cut makes (the last few: the round-robin over 8
