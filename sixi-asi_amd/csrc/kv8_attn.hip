@@ -84,10 +84,8 @@ __device__ __forceinline__ int blocks_of(const Lens& n) { return (n.cells + kBlk
 
 // How a call's cells are cut: pieces of c blocks, numbered stream by stream.  c is the work of
 // all streams over the work-groups asked for; nothing is cut where the tiles alone are nearly enough of
-// them.  Whole numbers, formed alike by every work-group of a call and of its merge.
-struct Place {
-    int s, tiles, pieces, at;  // stream, its tiles, pieces of each, number of its first piece
-};
+// them.  Whole numbers, formed alike by every work-group of a call.
+typedef Kv8Place Place;
 struct Cut {
     int c, total;
     // of the lane's stream (S <= 64), else of the last 64 looked at
@@ -136,8 +134,8 @@ struct Cut {
             c = (int)((float)c * fminf((float)total / (float)a.target, 1.5f)) / 2 * 2 + 2;
         }
     }
-    // The stream that holds piece `id`, or (by_stream) the place of stream `id`.
-    __device__ __forceinline__ Place find(const Kv8AttnArgs& a, int id, bool by_stream) {
+    // The stream that holds piece `id`.
+    __device__ __forceinline__ Place find(const Kv8AttnArgs& a, int id) {
         const int lane = threadIdx.x & 63, sum = total;
         Place p{0, 1, 1, 0};
         int before = 0;
@@ -148,7 +146,7 @@ struct Cut {
                 count(a, t, blocks, before);
                 before = total;
             }
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(by_stream ? s0 + lane == id : id >= at && id < at + mine);
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(id >= at && id < at + mine);
             if (hit) {
                 const int l = __builtin_ctzll(hit);
                 p.s = s0 + l;
@@ -337,7 +335,8 @@ __device__ __forceinline__ bool work_of(const Kv8AttnArgs& a, Work& w) {
     cut.begin(a);
     w.id = blockIdx.x;
     if (w.id >= cut.total) return false;
-    const Place p = cut.find(a, w.id, false);
+    const Place p = cut.find(a, w.id);
+    if (a.cut && w.id == p.at && threadIdx.x == 0) a.places[p.s] = p;  // for the merge
     w.s = p.s;
     w.pieces = p.pieces;
     const int x = w.id - p.at;
@@ -601,32 +600,92 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
         r.leave(a.part + ((int64_t)w.id * NW + wave) * tile_floats(D));
 }
 
-// Joins the pieces of 32 rows: D/32 work-groups of 256 threads, each with 4 of the accumulators' D/8 quads.
+// Joins the pieces of 32 rows: D/32 work-groups of four waves, each with 4 of the accumulators' D/8 quads.  What a
+// call's pieces left was written on other XCDs and comes from memory, so everything a wave needs is asked for at
+// once: up to 8 pieces by a wave for each quad, more by all four waves for all four quads, joined in LDS.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a) {
+    __shared__ __align__(16) kv8_f32x4 sums[kWaves][4][64];
+    __shared__ float tops[kWaves][32], totals[kWaves][32];
     const int s = blockIdx.z, g = blockIdx.y, quads = blockIdx.x % (D / 32), t32 = blockIdx.x / (D / 32);
-    Cut cut;
-    cut.begin(a);
-    const Place p = cut.find(a, s, true);
     const Lens len = lens_of(a, s);
     const int M = len.rows * a.G;
-    if (t32 * 32 >= M || p.pieces == 1) return;
-    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, quad = quads * 4 + (threadIdx.x >> 6);
-    const int rr = t32 * 32 + n;
-    if (rr >= M) return;
+    if (t32 * 32 >= M) return;
+    const Place p = a.places[s];
+    if (p.pieces == 1) return;
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int quad = quads * 4 + wave, rr = t32 * 32 + n;
+    const bool live = rr < M;
     const int64_t step = (int64_t)a.Hkv * a.waves * tile_floats(D);  // from piece to piece
     const float* at = a.part + (((int64_t)p.at + (int64_t)(p.tiles - 1 - t32 / a.waves) * p.pieces * a.Hkv + g) * a.waves + t32 % a.waves) * tile_floats(D);
-    float m = kLowest;
-#pragma unroll 8
-    for (int i = 0; i < p.pieces; ++i) m = fmaxf(m, at[i * step + 32 * D + n]);
-    float l = 0.0f;
+    float m = kLowest, l = 0.0f;
     kv8_f32x4 o = {};
-#pragma unroll 8
-    for (int i = 0; i < p.pieces; ++i) {
-        const float f = __builtin_amdgcn_exp2f(at[i * step + 32 * D + n] - m);
-        l = fmaf(at[i * step + 32 * D + 32 + n], f, l);
-        o += *reinterpret_cast<const kv8_f32x4*>(at + i * step + (quad * 64 + lane) * 4) * f;
+    if (p.pieces <= 8) {
+        float ms[8], ls[8];
+        kv8_f32x4 os[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const bool on = live && i < p.pieces;
+            ms[i] = on ? at[i * step + 32 * D + n] : kLowest;
+            ls[i] = on ? at[i * step + 32 * D + 32 + n] : 0.0f;
+            os[i] = on ? *reinterpret_cast<const kv8_f32x4*>(at + i * step + (quad * 64 + lane) * 4) : kv8_f32x4{};
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, ms[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = __builtin_amdgcn_exp2f(ms[i] - m);
+            l = fmaf(ls[i], f, l);
+            o += os[i] * f;
+        }
+    } else {
+        kv8_f32x4 x[4] = {};
+        for (int i0 = wave; i0 < p.pieces; i0 += 4 * kWaves) {
+            float ms[4], ls[4];
+            kv8_f32x4 os[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int i = i0 + k * kWaves;
+                const bool on = live && i < p.pieces;
+                ms[k] = on ? at[i * step + 32 * D + n] : kLowest;
+                ls[k] = on ? at[i * step + 32 * D + 32 + n] : 0.0f;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    os[k][q] = on ? *reinterpret_cast<const kv8_f32x4*>(at + i * step + ((quads * 4 + q) * 64 + lane) * 4) : kv8_f32x4{};
+            }
+            const float up = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), m), f0 = __builtin_amdgcn_exp2f(m - up);
+            m = up;
+            l *= f0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] *= f0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float f = __builtin_amdgcn_exp2f(ms[k] - m);
+                l = fmaf(ls[k], f, l);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) x[q] += os[k][q] * f;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) sums[wave][q][lane] = x[q];
+        if (h == 0) {
+            tops[wave][n] = m;
+            totals[wave][n] = l;
+        }
+        __syncthreads();
+        m = kLowest;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) m = fmaxf(m, tops[k][n]);
+        l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) {
+            const float f = __builtin_amdgcn_exp2f(tops[k][n] - m);
+            l = fmaf(totals[k][n], f, l);
+            o += sums[k][wave][lane] * f;
+        }
     }
+    if (!live) return;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     const int j = rr / a.G, head = g * a.G + rr % a.G;
     store4(a, a.out + (int64_t)head * a.o_nb1 + (int64_t)j * a.o_nb2 + (int64_t)s * a.o_nb3, quad / 4 * 32 + quad % 4 * 8 + 4 * h, o * inv);
@@ -672,7 +731,8 @@ size_t kv8_attn_plan(Kv8AttnArgs& a) {
     a.grid = (int32_t)(tiles + (a.cut ? a.target : 0) + 16);
     if (!a.cut) return 256;
     const int64_t slots = (tiles < a.target ? tiles : a.target) + a.target + 16;
-    return ((size_t)slots * a.waves * tile_floats(a.D) * sizeof(float) + 255) / 256 * 256;
+    a.places = reinterpret_cast<Kv8Place*>(a.part + slots * a.waves * tile_floats(a.D));
+    return ((size_t)slots * a.waves * tile_floats(a.D) * sizeof(float) + (size_t)a.S * sizeof(Kv8Place) + 255) / 256 * 256;
 }
 
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t stream) {

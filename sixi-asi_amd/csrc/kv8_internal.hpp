@@ -44,6 +44,11 @@ struct Kv8RowsArgs {
 hipError_t launch_kv8_write(const Kv8RowsArgs& a, hipStream_t stream);
 hipError_t launch_kv8_read(const Kv8RowsArgs& a, hipStream_t stream);
 
+// Where the pieces of a stream's cells begin.
+struct Kv8Place {
+    int32_t s, tiles, pieces, at;  // stream, its tiles, pieces of each, number of its first piece
+};
+
 struct Kv8AttnArgs {
     const char* q;
     int64_t q_nb1, q_nb2, q_nb3;  // row, head, stream
@@ -61,7 +66,8 @@ struct Kv8AttnArgs {
     int32_t S, H, Hkv, G, n_q, n_kv, D;
     float scale_log2;             // |scale| * log2(e); the sign goes into Q
     float q_sign;
-    float* part;                  // workspace
+    float* part;                  // workspace: partial results of the pieces
+    Kv8Place* places;             // and, behind them, each stream's place
     int32_t waves;                // row tiles of 32 that a work-group takes (1: its waves share the cells)
     int32_t target;               // work-groups that the cells are cut for
     int32_t least;                // blocks of a piece at least

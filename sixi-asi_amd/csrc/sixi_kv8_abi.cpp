@@ -225,8 +225,8 @@ int resolve_attn(const sixi_kv8_attn_params* p, sixi::Kv8AttnArgs* out, size_t* 
     a.scale_log2 = std::fmax(std::fabs(p->scale) * 1.4426950408889634f, 0x1p-85f);
     a.q_sign = std::signbit(p->scale) ? -1.0f : 1.0f;
     if ((a.n_q * (int64_t)a.G + 31) / 32 * a.Hkv * S > ((int64_t)1 << 28)) return SIXI_E_UNSUPPORTED;  // work-groups
-    *ws = sixi::kv8_attn_plan(a);
     a.part = static_cast<float*>(p->workspace);
+    *ws = sixi::kv8_attn_plan(a);
     *out = a;
     return SIXI_OK;
 }
