@@ -457,6 +457,18 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
 
 // Four waves of 32 rows each over the same cells, NB blocks of 32 a step.  A wave without rows still converts
 // its share of the codes: three waves of rows and one without measured faster than a work-group of three.
+// N products whose left operands come from LDS: six reads first, then two more with every two products, so that a
+// read has the time of four products to arrive.
+template <int N>
+__device__ __forceinline__ void feed() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+}
+
 template <int D, int NB>
 constexpr size_t rows_lds() {
     return (size_t)2 * 2 * NB * (D / 32) * 2 * 64 * 16;
@@ -534,41 +546,45 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                 es[i] = (float)e0[i];
             }
         };
-        // One step.  EDGE: some row may not see every cell.  The products run at a raised priority, so that
-        // the matrix cores serve one wave of a SIMD while the other is at its softmax.
-        auto step = [&](int b, auto BUF, auto EDGE) {
+        // One step.  The products run at a raised priority, so that the matrix cores serve one wave of a SIMD
+        // while the other is at its softmax.
+        auto step = [&](int b, auto BUF) {
             constexpr int buf = decltype(BUF)::value;
             load();  // (behind the last step: its blocks once more, and not used)
-            if (!decltype(EDGE)::value || b * kBlk < r.reach) {
+            if (b * kBlk < r.reach) {
                 f32x16 sc[NB] = {};
                 kv8_f16x8 p[NB][2];
+                __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-                for (int i = 0; i < NB; ++i)
+                for (int c = 0; c < KC; ++c)
 #pragma unroll
-                    for (int c = 0; c < KC; ++c) {
-                        sc[i] = mfma(tile[buf][0][i * KC + c][0][lane], r.q[c][0], sc[i]);
-                        sc[i] = mfma(tile[buf][0][i * KC + c][1][lane], r.q[c][1], sc[i]);
-                    }
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < NB; ++i) sc[i] = mfma(tile[buf][0][i * KC + c][u][lane], r.q[c][u], sc[i]);
+                feed<2 * NB * KC>();
                 __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
                 float top = kLowest;
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
-                    if (decltype(EDGE)::value) r.template hide<MASK>(a, sc[i], b + i, ks[i], es[i], mask);
+                    r.template hide<MASK>(a, sc[i], b + i, ks[i], es[i], mask);
                     top = __builtin_elementwise_maximum(top, r.template top_of<MASK>(sc[i], ks[i], es[i]));
                 }
                 r.raise(top);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) r.template weights<MASK>(sc[i], ks[i], es[i], e0[i], p[i]);
+                __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int i = 0; i < NB; ++i)
 #pragma unroll
-                    for (int c = 0; c < KC; ++c) {
-                        r.o[c] = mfma(tile[buf][1][i * KC + c][0][lane], p[i][0], r.o[c]);
-                        r.o[c] = mfma(tile[buf][1][i * KC + c][1][lane], p[i][1], r.o[c]);
-                    }
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int c = 0; c < KC; ++c) r.o[c] = mfma(tile[buf][1][i * KC + c][u][lane], p[i][u], r.o[c]);
+                feed<2 * NB * KC>();
                 __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
             }
             convert(buf ^ 1);
             __syncthreads();
@@ -577,20 +593,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
         load();
         convert(0);
         __syncthreads();
-        // steps in pairs, one for each buffer; first those whose cells every row of the work-group sees
+        // steps in pairs, one for each buffer.  (A loop of its own for the steps whose cells every row sees took
+        // 50 more registers, and with them the reads ahead: 203 against 1xx us for the prompt chunk.)
         using std::integral_constant;
-        const int sees = a.mode == SIXI_MASK_BLOCK_CAUSAL ? w.n.cached + r0 / a.G + 1 : w.n.cells;
-        const int plain = MASK || r0 + 32 * NW > w.n.rows * a.G ? w.first : min(last, sees / kBlk);
-        int b = w.first;
 #pragma unroll 1
-        for (; b + 2 * NB <= plain; b += 2 * NB) {
-            step(b, integral_constant<int, 0>{}, integral_constant<bool, false>{});
-            step(b + NB, integral_constant<int, 1>{}, integral_constant<bool, false>{});
-        }
-#pragma unroll 1
-        for (; b < last; b += 2 * NB) {
-            step(b, integral_constant<int, 0>{}, integral_constant<bool, true>{});
-            if (b + NB < last) step(b + NB, integral_constant<int, 1>{}, integral_constant<bool, true>{});
+        for (int b = w.first; b < last; b += 2 * NB) {
+            step(b, integral_constant<int, 0>{});
+            if (b + NB < last) step(b + NB, integral_constant<int, 1>{});
         }
     }
     r.l = sum_halves(r.l);
