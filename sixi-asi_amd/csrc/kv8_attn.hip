@@ -457,11 +457,11 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
 
 // Four waves of 32 rows each over the same cells, NB blocks of 32 a step.  A wave without rows still converts
 // its share of the codes: three waves of rows and one without measured faster than a work-group of three.
-// N products whose left operands come from LDS: six reads first, then two more with every two products, so that a
-// read has the time of four products to arrive.
-template <int N>
+// N products whose left operands come from LDS: A reads first, then two more with every two products, so that a
+// read has the time of A - 2 products to arrive.
+template <int N, int A>
 __device__ __forceinline__ void feed() {
-    __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, A, 0);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
         __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
@@ -477,7 +477,9 @@ constexpr size_t rows_lds() {
 template <int D, int NB, bool MASK>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnArgs a) {
     constexpr int NW = kWaves;
-    constexpr int KC = D / 32, ITEMS = NB * KC, MINE = (ITEMS + NW - 1) / NW;
+    constexpr int KC = D / 32, ITEMS = NB * KC, MINE = ITEMS / NW;
+    constexpr int kAhead = D == 128 ? 6 : 4;  // LDS reads ahead of their products
+    static_assert(ITEMS % NW == 0, "every wave converts the same share");
     extern __shared__ __align__(16) float lds[];
     // [buffer][K, V][block, piece][first, second eight][lane] 8 f16
     typedef kv8_f16x8 Tile[2][ITEMS][2][64];
@@ -496,49 +498,49 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
     if (w.first < last) {
         const uint32_t k_off = h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
         const uint32_t v_off = n * kBlk + h * 16;
-        // the wave's share of the next step's codes, on their way
-        kv8_u32x4 kc[MINE], vc[MINE];
+        // The wave's share of the next step's codes, on their way.  At 256 dims K and V go through the same
+        // registers, K in the first half of a step and V in the second.
+        constexpr bool kOne = D == 256;
+        kv8_u32x4 codes[kOne ? 1 : 2][MINE];
         int ek[NB], ev[NB];
         BlockWalk walk;
-        auto fetch = [&](kv8_u32x4 (&codes)[MINE], const char* p, uint32_t off, int32_t step) {
-#pragma unroll
-            for (int i = 0; i < MINE; ++i) {
-                const int it = min(wave + i * NW, ITEMS - 1);
-                codes[i] = *reinterpret_cast<const kv8_u32x4*>(p + ((NB > 1 && it >= KC ? step : 0) + it % KC * (kBlk * 32)) + off);
-            }
-        };
         // the walk's step; a second block that is none is the first once more (its cells are hidden).  The
         // compiler is not to know that: it would wait for the first one's exponents to copy them.
-        auto load = [&]() {
+        auto load = [&](int which) {
             const bool both = walk.b + 1 < last;
-            int k_step = both ? walk.k_nb : 0, v_step = both ? walk.v_nb : 0;
+            int step = both ? (which ? walk.v_nb : walk.k_nb) : 0;
+            asm("" : "+s"(step));
+            const char* p = which ? walk.v : walk.k;
+            const uint32_t off = which ? v_off : k_off;
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+                const int it = wave + i * NW;
+                codes[kOne ? 0 : which][i] = *reinterpret_cast<const kv8_u32x4*>(p + ((NB > 1 && it >= KC ? step : 0) + it % KC * (kBlk * 32)) + off);
+            }
+        };
+        auto load_exps = [&]() {
+            const bool both = walk.b + 1 < last;
             int ke_step = both ? walk.ke_nb : 0, ve_step = both ? walk.ve_nb : 0;
-            asm("" : "+s"(k_step), "+s"(v_step), "+s"(ke_step), "+s"(ve_step));
-            fetch(kc, walk.k, k_off, k_step);
-            fetch(vc, walk.v, v_off, v_step);
+            asm("" : "+s"(ke_step), "+s"(ve_step));
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 ek[i] = walk.ke[i * ke_step];
                 ev[i] = walk.ve[i * ve_step];
             }
-            walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
         };
         float ks[NB], es[NB];
         int e0[NB];
-        // the codes as f16 into a buffer
-        auto convert = [&](int buf) {
+        // codes as f16 into a buffer
+        auto convert = [&](int buf, int which) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-                for (int i = 0; i < MINE; ++i) {
-                    const int it = wave + i * NW;
-                    if (ITEMS % NW == 0 || it < ITEMS) {
-                        kv8_f16x8 x, y;
-                        codes_f16x16(k ? vc[i] : kc[i], x, y);
-                        tile[buf][k][it][0][lane] = x;
-                        tile[buf][k][it][1][lane] = y;
-                    }
-                }
+            for (int i = 0; i < MINE; ++i) {
+                kv8_f16x8 x, y;
+                codes_f16x16(codes[kOne ? 0 : which][i], x, y);
+                tile[buf][which][wave + i * NW][0][lane] = x;
+                tile[buf][which][wave + i * NW][1][lane] = y;
+            }
+        };
+        auto scales = [&]() {
 #pragma unroll
             for (int i = 0; i < NB; ++i) {
                 ks[i] = a.scale_log2 * exp2_int(clamp_exp(ek[i]));
@@ -550,10 +552,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
         // while the other is at its softmax.
         auto step = [&](int b, auto BUF) {
             constexpr int buf = decltype(BUF)::value;
-            load();  // (behind the last step: its blocks once more, and not used)
-            if (b * kBlk < r.reach) {
-                f32x16 sc[NB] = {};
-                kv8_f16x8 p[NB][2];
+            const bool any = b * kBlk < r.reach;
+            f32x16 sc[NB] = {};
+            // (behind the last step: its blocks once more, and not used)
+            if (!kOne) {
+                load(0);
+                load(1);
+                load_exps();
+                walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
+            }
+            if (any) {
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -562,9 +570,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int i = 0; i < NB; ++i) sc[i] = mfma(tile[buf][0][i * KC + c][u][lane], r.q[c][u], sc[i]);
-                feed<2 * NB * KC>();
+                feed<2 * NB * KC, kAhead>();
                 __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
+            }
+            if (kOne) {
+                convert(buf ^ 1, 0);
+                load(1);
+                load_exps();
+                walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
+            }
+            if (any) {
+                kv8_f16x8 p[NB][2];
                 float top = kLowest;
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
@@ -582,16 +599,25 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int c = 0; c < KC; ++c) r.o[c] = mfma(tile[buf][1][i * KC + c][u][lane], p[i][u], r.o[c]);
-                feed<2 * NB * KC>();
+                feed<2 * NB * KC, kAhead>();
                 __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            convert(buf ^ 1);
+            if (!kOne) convert(buf ^ 1, 0);
+            convert(buf ^ 1, 1);
+            scales();
+            if (kOne) load(0);
             __syncthreads();
         };
         walk.begin(a.pages, a.k, a.v, w.s, w.g, w.first, last);
-        load();
-        convert(0);
+        load(0);
+        load_exps();
+        convert(0, 0);
+        load(1);
+        convert(0, 1);
+        scales();
+        walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
+        if (kOne) load(0);
         __syncthreads();
         // steps in pairs, one for each buffer.  (A loop of its own for the steps whose cells every row sees took
         // 50 more registers, and with them the reads ahead: 203 against 1xx us for the prompt chunk.)
