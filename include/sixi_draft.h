@@ -53,7 +53,7 @@ typedef struct sixi_draft_params {
 } sixi_draft_params;
 
 /* Decides every stream.  A logit of -inf or NaN has no weight (a sampler's filters strike tokens so);
- * +inf takes all.  If p - q leaves no weight, the draw is from p. */
+ * +inf takes all.  A NaN temperature counts as 0.  If p - q leaves no weight, the draw is from p. */
 int sixi_draft_verify(const sixi_draft_params* p);
 
 int sixi_draft_workspace_bytes(const sixi_draft_params* p, size_t* bytes);

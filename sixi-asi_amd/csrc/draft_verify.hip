@@ -42,7 +42,7 @@ __device__ __forceinline__ double exp2_neg(double y) {
 // exp((l - top) / T) with c = log2(e) / T; 0 for -inf and NaN.  Where the top is infinite, its equals take all.
 __device__ __forceinline__ double weight(float l, float top, double c) {
     if (top == __builtin_huge_valf()) return l == top ? 1.0 : 0.0;
-    return exp2_neg(fma((double)l, c, -(double)top * c));
+    return exp2_neg(((double)l - (double)top) * c);
 }
 
 __device__ __forceinline__ float load1(const char* p, int type) {
@@ -53,7 +53,11 @@ __device__ __forceinline__ float load1(const char* p, int type) {
 }
 __device__ __forceinline__ int bytes_of(int type) { return type == SIXI_TYPE_F32 ? 4 : 2; }
 
-__device__ __forceinline__ float heat_of(const DraftArgs& a, int s) { return a.temperature ? a.temperature[s] : 1.0f; }
+// A stream's temperature: 0 for a greedy one (NaN too), at most the largest finite number.
+__device__ __forceinline__ float heat_of(const DraftArgs& a, int s) {
+    const float t = a.temperature ? a.temperature[s] : 1.0f;
+    return t > 0.0f ? fminf(t, 3.4028235e38f) : 0.0f;
+}
 __device__ __forceinline__ int rows_of(const DraftArgs& a, int s) {
     return a.q_len ? min(max(a.q_len[s], 0), a.n_rows) : a.n_rows;
 }
@@ -230,7 +234,13 @@ __global__ __launch_bounds__(kThreads) void draft_rows_kernel(DraftArgs a) {
                 sum *= weight(top, here, c);
                 top = here;
             }
-            sum += sum_of(x, top, c, top - span);
+            // (temperatures whose 1000 powers of two are a few steps of the top, or past the type: one by one)
+            if (span >= fabsf(top) * 0x1p-18f && span < 1e30f && fabsf(top) < 1e30f) {
+                sum += sum_of(x, top, c, top - span);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) sum += weight(x[i], top, c);
+            }
         }
     }
     sum = wave_reduce(sum, Plus());
@@ -356,10 +366,9 @@ __device__ __forceinline__ void weights_of(const DraftArgs& a, int s, const Draf
     }
     // (no branch between the tokens: their polynomials run next to one another)
     const bool all = v.top == __builtin_huge_valf();
-    const double off = all ? 0.0 : -(double)v.top * v.c;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-        double y = fma((double)x[i], v.c, off);
+        double y = ((double)x[i] - (double)v.top) * v.c;
         if (all) y = x[i] == v.top ? 0.0 : -2000.0;
         p[i] = exp2_neg(y) * v.inv_z;  // (0 past the end: -inf there)
     }

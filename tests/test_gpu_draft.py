@@ -49,7 +49,8 @@ def _rule(logits, draft, u, u_next, rows, heat, probs):
             known = 0 <= d < V
             q = (probs[j] if probs is not None else np.eye(1, V, d)[0]) if known or probs is not None else np.zeros(V)
             left, right = float(u[j]) * (float(q[d]) if known else 1.0), float(p[d]) if known else 0.0
-            assert left == right or abs(left - right) > 1e-9
+            # no rounding decides: apart, equal, or 0 against a weight that 64 bits hold (p > 0 however it is formed)
+            assert left == right or abs(left - right) > 1e-9 or left == 0 and right > 1e-250
             if left < right:
                 j += 1
                 continue
@@ -175,6 +176,22 @@ def test_draft_verify_extremes():
     assert list(got) == want
     assert got[0][0] == 1 and got[1][0] == -1
     assert got[0][3:6] == [1, 1, 1] and got[0][8] == 1 and got[1][8] == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_draft_verify_temperatures(dtype):
+    """From the smallest number of the type to the largest, the logits far from 0: what differs by more than 1000 powers of
+    two from the top has no weight, whatever steps f32 has there; at the largest, what is not struck weighs alike.  NaN is
+    greedy, as 0."""
+    heats = [1e-40, 1e-30, 1e-12, 1e-9, 2e-8, 1e-7, 3e-7, 1e-6, 1e-5, 1e-3, 30.0, 1e6, 1e20, 1e33, 3e38, float("nan"), 0.0]
+    for shift in (0.0, 100.0, -5000.0):
+        c = _case(len(heats), 3, 9000, False, 31, dtype=dtype)
+        c["heat"] = np.array(heats, np.float32)
+        c["logits"] = (c["logits"].float() + shift).to(dtype)
+        c["u"][:] = np.linspace(0.001, 0.3, c["u"].size, dtype=np.float32).reshape(c["u"].shape)
+        with np.errstate(over="ignore"):
+            want = _want(c)
+        assert list(_run(c)) == want, shift
 
 
 def test_draft_verify_where_p_minus_q_leaves_nothing():
