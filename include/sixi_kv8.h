@@ -76,7 +76,8 @@ typedef struct sixi_kv8_rows_params {
  *   - the kept cells' codes become the nearest multiples of the new scale (ties to even): a
  *     scale grows as louder rows arrive, and starts anew when a block is written from its first
  *     cell.  The bytes of cells behind the last row do not change.
- * Infinities are stored as +-127 * 2^e, NaN as 0. */
+ * Infinities are stored as +-127 * 2^e, NaN as 0.  A block is written whole: streams that share a
+ * page must not store into the same block of it in one call, nor in calls that may overlap. */
 int sixi_kv8_write(const sixi_kv8_rows_params* p);
 
 /* Reads cell kv_len[s] + j into row j < q_len[s] of k and v.  Exact in f32; f16 rows hold the
@@ -117,8 +118,9 @@ typedef struct sixi_kv8_attn_params {
  * q_len[s]: decode, verify and prefill by the row count.  q-heads g*G .. g*G+G-1 share kv-head g
  * (G = H / Hkv, any ratio).  The cells a row sees are those of sixi_attn_params.mask_mode; kv_len[s]
  * is clamped to [0, n_kv - q_len[s]] on the device.  A row that sees no cell is zero; rows
- * j >= q_len[s] are not written.  Q K^T and the sums run in f32 over exact products; the softmax's
- * weights are rounded to f16 in front of the product with V. */
+ * j >= q_len[s] are not written.  Q K^T and the sums run in f32 over exact products of the codes and
+ * Q in f16 (an f32 Q is rounded to f16 as it is read); the softmax's weights are rounded to f16 in
+ * front of the product with V.  At most 2^23 tiles of 32 rows (n_q * G of a head) in a call. */
 int sixi_kv8_attn(const sixi_kv8_attn_params* p);
 
 /* Workspace the call needs for this description (not dependent on the device-side lengths). */

@@ -70,7 +70,8 @@ typedef struct sixi_qk_rope_params {
  *   (x0, x1) -> mscale * (x0 cos a - x1 sin a, x1 cos a + x0 sin a)
  * after x = x / sqrt(mean(x^2) + eps) * norm where norm weights are given.  Dims past n_rot pass
  * (normed, unscaled).  Angles are reduced in 64 bits.  D is a multiple of 16 up to 256; rows, weights
- * and strides 16-byte aligned.  Rows past q_len are not written. */
+ * and strides 16-byte aligned.  Rows past q_len are not written.  At most 2^23 rows of a stream and
+ * 65535 heads and streams. */
 int sixi_qk_rope(const sixi_qk_rope_params* p);
 
 /* Host-side validation only: SIXI_OK or the error sixi_qk_rope returns. */

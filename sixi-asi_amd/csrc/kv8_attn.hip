@@ -25,6 +25,7 @@
 // Work-groups: every stream's cells are cut into pieces of c blocks, c from the lengths on the device, so
 // that streams of any lengths fill the chip; pieces of one (stream, head, tile) are joined by a second
 // launch in their order.
+#include <algorithm>
 #include <type_traits>
 
 #include "device_util.hpp"
@@ -82,6 +83,11 @@ __device__ __forceinline__ Lens lens_of(const Kv8AttnArgs& a, int s) {
 }
 __device__ __forceinline__ int blocks_of(const Lens& n) { return (n.cells + kBlk - 1) / kBlk; }
 
+// Whether tiles are nearly a work-group for every place there is: then no cells are cut.
+__device__ __host__ __forceinline__ bool enough(int64_t tiles, const Kv8AttnArgs& a) {
+    return 4 * tiles * a.Hkv >= 3 * (int64_t)a.target;
+}
+
 // How a call's cells are cut: pieces of c blocks, numbered stream by stream.  c is the work of
 // all streams over the work-groups asked for; nothing is cut where the tiles alone are nearly enough of
 // them.  Whole numbers, formed alike by every work-group of a call.
@@ -111,15 +117,15 @@ struct Cut {
         const int lane = threadIdx.x & 63;
         int t = 0, blocks = 0, all = 0, work = 0;
         // a stream's share of a work-group's blocks, in 1/64 (f32, and then whole numbers: the same sum in
-        // every work-group; kept in range for sums of 512)
+        // every work-group; where cells are cut it is at most 0.75 * 64 * 2^21 blocks in all)
         const float unit = 64.0f * (float)a.Hkv / (float)a.target;
         for (int s0 = 0; s0 < a.S; s0 += 64) {
             stream(a, s0 + lane, t, blocks);
             all += __builtin_amdgcn_readlane(wave_scan(t), 63);
-            work += __builtin_amdgcn_readlane(wave_scan((int)fminf((float)t * (float)blocks * unit, 4194303.0f) + 1), 63);
+            work += __builtin_amdgcn_readlane(wave_scan((int)fminf((float)t * (float)blocks * unit, 134217728.0f) + 1), 63);
         }
         // even: two blocks a step, and of one page
-        c = (float)all * (float)a.Hkv >= 0.75f * (float)a.target ? 1 << 26 : (max((work + 63) / 64, a.least) + 1) / 2 * 2;
+        c = enough(all, a) ? 1 << 26 : (max((work + 63) / 64, a.least) + 1) / 2 * 2;
         // every stream's last piece is a part of one: longer pieces until they fit the places there are
         for (int tries = 0;; ++tries) {
             total = 0;
@@ -620,7 +626,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
         if (kOne) load(0);
         __syncthreads();
         // steps in pairs, one for each buffer.  (A loop of its own for the steps whose cells every row sees took
-        // 50 more registers, and with them the reads ahead: 203 against 1xx us for the prompt chunk.)
+        // 50 more registers, and with them the reads ahead: 203 against 182 us for the prompt chunk.)
         using std::integral_constant;
 #pragma unroll 1
         for (int b = w.first; b < last; b += 2 * NB) {
@@ -746,7 +752,8 @@ hipError_t launch(const Kv8AttnArgs& a, hipStream_t stream) {
         launch_pieces<D, false>(a, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !a.cut) return e;
-    const int64_t t32 = ((int64_t)a.n_q * a.G + 31) / 32;
+    // (a cut stream has fewer tiles than make 3/4 of the target over the heads)
+    const int64_t t32 = std::min(((int64_t)a.n_q * a.G + 31) / 32, (3 * (int64_t)a.target / (4 * a.Hkv) + 1) * a.waves);
     hipLaunchKernelGGL(kv8_merge_kernel<D>, dim3((unsigned)(t32 * (D / 32)), (unsigned)a.Hkv, (unsigned)a.S), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
@@ -762,11 +769,12 @@ size_t kv8_attn_plan(Kv8AttnArgs& a) {
     const int64_t blocks = (a.n_kv + kBlk - 1) / kBlk;
     // pieces at most: one for each tile, and those that a cut makes (the last few: the round-robin over 8
     // XCDs, and f32 sums of large numbers); a cut is made only over fewer tiles than 3/4 of the target
-    a.cut = blocks > a.least;
+    // (none where the host can tell that the tiles are enough: then there is nothing to join)
+    a.cut = blocks > a.least && (a.q_len || !enough(tiles / a.Hkv, a));
     a.grid = (int32_t)(tiles + (a.cut ? a.target : 0) + 16);
     if (!a.cut) return 256;
     const int64_t slots = (tiles < a.target ? tiles : a.target) + a.target + 16;
-    a.places = reinterpret_cast<Kv8Place*>(a.part + slots * a.waves * tile_floats(a.D));
+    if (a.part) a.places = reinterpret_cast<Kv8Place*>(a.part + slots * a.waves * tile_floats(a.D));
     return ((size_t)slots * a.waves * tile_floats(a.D) * sizeof(float) + (size_t)a.S * sizeof(Kv8Place) + 255) / 256 * 256;
 }
 

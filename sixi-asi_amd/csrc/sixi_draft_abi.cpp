@@ -104,8 +104,10 @@ int resolve(const sixi_draft_params* p, sixi::DraftArgs* out, size_t* ws) {
     *ws = (*ws + 255) / 256 * 256;
     if (*ws == 0) *ws = 256;
     a.parts = static_cast<sixi::DraftPart*>(p->workspace);
-    a.draws = reinterpret_cast<sixi::DraftDraw*>(static_cast<char*>(p->workspace) + parts);
-    a.counts = reinterpret_cast<int32_t*>(static_cast<char*>(p->workspace) + parts + draws);
+    if (p->workspace) {
+        a.draws = reinterpret_cast<sixi::DraftDraw*>(static_cast<char*>(p->workspace) + parts);
+        a.counts = reinterpret_cast<int32_t*>(static_cast<char*>(p->workspace) + parts + draws);
+    }
     *out = a;
     return SIXI_OK;
 }
@@ -140,6 +142,11 @@ int sixi_draft_verify(const sixi_draft_params* p) {
         ranges_overlap(p->workspace, (int64_t)ws, p->keep, a.S * 4) || ranges_overlap(p->workspace, (int64_t)ws, p->token, a.S * 4) ||
         (a.probs && ranges_overlap(p->workspace, (int64_t)ws, a.probs,
                                    view_span(p->draft_probs, p->draft_probs.ne[0] * type_bytes(a.p_type)))))
+        return SIXI_E_INVALID_ARGUMENT;
+    for (const void* r : {(const void*)p->u_next, (const void*)p->temperature, (const void*)p->q_len})
+        if (r && ranges_overlap(p->workspace, (int64_t)ws, r, a.S * 4)) return SIXI_E_INVALID_ARGUMENT;
+    if (a.n_rows > 1 && (ranges_overlap(p->workspace, (int64_t)ws, a.draft, ((a.S - 1) * a.draft_stride + a.n_rows - 1) * 4) ||
+                         ranges_overlap(p->workspace, (int64_t)ws, a.u, ((a.S - 1) * a.u_stride + a.n_rows - 1) * 4)))
         return SIXI_E_INVALID_ARGUMENT;
     return sixi::launch_draft_verify(a, static_cast<hipStream_t>(p->stream)) == hipSuccess ? SIXI_OK : SIXI_E_BACKEND;
 }

@@ -44,8 +44,8 @@ int check_cache(const sixi_kv8_cache& c, bool paged, CacheViews* out) {
     for (int i = 0; i < 3; ++i) {
         if (c.k_nb[i] < 0 || c.v_nb[i] < 0 || c.k_exp_nb[i] < 0 || c.v_exp_nb[i] < 0) return SIXI_E_INVALID_ARGUMENT;
         if (c.k_nb[i] % 16 || c.v_nb[i] % 16) return SIXI_E_ALIGNMENT;
-        if (i == 0 && (c.k_nb[0] > INT32_MAX || c.v_nb[0] > INT32_MAX || c.k_exp_nb[0] > INT32_MAX || c.v_exp_nb[0] > INT32_MAX))
-            return SIXI_E_UNSUPPORTED;  // (steps from block to block are 32-bit)
+        const int64_t most = INT32_MAX / 2;  // (steps from block to block are 32-bit)
+        if (i == 0 && (c.k_nb[0] > most || c.v_nb[0] > most || c.k_exp_nb[0] > most || c.v_exp_nb[0] > most)) return SIXI_E_UNSUPPORTED;
     }
     if (!aligned(c.k, 16) || !aligned(c.v, 16)) return SIXI_E_ALIGNMENT;
     const int64_t bytes = (int64_t)sixi::kBlk * c.head_dim;
@@ -79,6 +79,13 @@ sixi::Kv8Tensor tensor_of(void* codes, int8_t* exps, const int64_t (&nb)[3], con
     return t;
 }
 
+// Whether a written range meets the lengths or the page table.
+template <typename P>
+bool meets_arrays(const void* w, int64_t bytes, const P& p, int64_t S) {
+    return (p.kv_len && ranges_overlap(w, bytes, p.kv_len, S * 4)) || (p.q_len && ranges_overlap(w, bytes, p.q_len, S * 4)) ||
+           (p.page_table && ranges_overlap(w, bytes, p.page_table, S * p.page_table_stride * 4));
+}
+
 int resolve_rows(const sixi_kv8_rows_params* p, bool read, sixi::Kv8RowsArgs* out) {
     if (!p || p->flags != 0) return SIXI_E_INVALID_ARGUMENT;
     const sixi_kv8_cache& c = p->cache;
@@ -106,7 +113,7 @@ int resolve_rows(const sixi_kv8_rows_params* p, bool read, sixi::Kv8RowsArgs* ou
         if (!aligned(r.data, 16)) return SIXI_E_ALIGNMENT;
         const int64_t rb = D * es;
         if (view_span(r, rb) < 0) return SIXI_E_INTEGER_OVERFLOW;
-        if (read && !rows_disjoint(r, rb)) return SIXI_E_INVALID_ARGUMENT;
+        if (read && view_span(r, rb) > 0 && (!rows_disjoint(r, rb) || meets_arrays(r.data, view_span(r, rb), *p, S))) return SIXI_E_INVALID_ARGUMENT;
         for (const sixi_view* v : {&cv.k, &cv.v, &cv.ke, &cv.ve})
             if (views_overlap(r, rb, *v, v->ne[0])) return SIXI_E_INVALID_ARGUMENT;
         a.rows[i] = static_cast<char*>(const_cast<void*>(r.data));
@@ -123,9 +130,11 @@ int resolve_rows(const sixi_kv8_rows_params* p, bool read, sixi::Kv8RowsArgs* ou
     } else {
         // four tensors written by different work-groups
         const sixi_view* w[4] = {&cv.k, &cv.v, &cv.ke, &cv.ve};
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
             for (int j = i + 1; j < 4; ++j)
                 if (views_overlap(*w[i], w[i]->ne[0], *w[j], w[j]->ne[0])) return SIXI_E_INVALID_ARGUMENT;
+            if (meets_arrays(w[i]->data, view_span(*w[i], w[i]->ne[0]), *p, S)) return SIXI_E_INVALID_ARGUMENT;
+        }
     }
     a.t[0] = tensor_of(c.k, c.k_exp, c.k_nb, c.k_exp_nb);
     a.t[1] = tensor_of(c.v, c.v_exp, c.v_nb, c.v_exp_nb);
@@ -171,10 +180,7 @@ int resolve_attn(const sixi_kv8_attn_params* p, sixi::Kv8AttnArgs* out, size_t* 
     if (!rows_disjoint(o, ob) || views_overlap(o, ob, q, qb)) return SIXI_E_INVALID_ARGUMENT;
     for (const sixi_view* v : {&cv.k, &cv.v, &cv.ke, &cv.ve})
         if (views_overlap(o, ob, *v, v->ne[0])) return SIXI_E_INVALID_ARGUMENT;
-    const int64_t span = view_span(o, ob);
-    if (ranges_overlap(o.data, span, p->kv_len, p->kv_len ? S * 4 : 0) || ranges_overlap(o.data, span, p->q_len, p->q_len ? S * 4 : 0) ||
-        ranges_overlap(o.data, span, p->page_table, paged ? S * p->page_table_stride * 4 : 0))
-        return SIXI_E_INVALID_ARGUMENT;
+    if (meets_arrays(o.data, view_span(o, ob), *p, S)) return SIXI_E_INVALID_ARGUMENT;
 
     const int mode = p->mask_mode;
     if (mode < SIXI_MASK_NONE || mode > SIXI_MASK_EXPLICIT) return SIXI_E_INVALID_ARGUMENT;
@@ -224,7 +230,7 @@ int resolve_attn(const sixi_kv8_attn_params* p, sixi::Kv8AttnArgs* out, size_t* 
     // a scale of 0 becomes one that no score can notice: hidden cells are -inf times it
     a.scale_log2 = std::fmax(std::fabs(p->scale) * 1.4426950408889634f, 0x1p-85f);
     a.q_sign = std::signbit(p->scale) ? -1.0f : 1.0f;
-    if ((a.n_q * (int64_t)a.G + 31) / 32 * a.Hkv * S > ((int64_t)1 << 28)) return SIXI_E_UNSUPPORTED;  // work-groups
+    if ((a.n_q * (int64_t)a.G + 31) / 32 * a.Hkv * S > ((int64_t)1 << 23)) return SIXI_E_UNSUPPORTED;  // work-groups
     a.part = static_cast<float*>(p->workspace);
     *ws = sixi::kv8_attn_plan(a);
     *out = a;
@@ -302,7 +308,8 @@ int sixi_kv8_attn(const sixi_kv8_attn_params* p) {
         if (ranges_overlap(p->workspace, (int64_t)ws, v->data, view_span(*v, v->ne[0]))) return SIXI_E_INVALID_ARGUMENT;
     if (ranges_overlap(p->workspace, (int64_t)ws, p->q.data, view_span(p->q, a.D * elem_bytes(p->q.type))) ||
         ranges_overlap(p->workspace, (int64_t)ws, p->out.data, view_span(p->out, a.D * elem_bytes(p->out.type))) ||
-        (a.mask && ranges_overlap(p->workspace, (int64_t)ws, p->mask.data, view_span(p->mask, p->mask.ne[0] * 2))))
+        (a.mask && ranges_overlap(p->workspace, (int64_t)ws, p->mask.data, view_span(p->mask, p->mask.ne[0] * 2))) ||
+        meets_arrays(p->workspace, (int64_t)ws, *p, a.S))
         return SIXI_E_INVALID_ARGUMENT;
     return sixi::launch_kv8_attn(a, static_cast<hipStream_t>(p->stream)) == hipSuccess ? SIXI_OK : SIXI_E_BACKEND;
 }

@@ -44,7 +44,7 @@ int check_pair(const sixi_view& in, const sixi_view& out, sixi::RopeTensor* t) {
     for (int i = 0; i < 4; ++i)
         if (in.ne[i] != out.ne[i]) return SIXI_E_INVALID_ARGUMENT;
     const int64_t ib = in.ne[0] * elem_bytes(in.type), ob = out.ne[0] * elem_bytes(out.type);
-    if (!rows_disjoint(out, ob)) return SIXI_E_INVALID_ARGUMENT;
+    if (view_span(out, ob) > 0 && !rows_disjoint(out, ob)) return SIXI_E_INVALID_ARGUMENT;
     // in place, row for row, or apart: a row is read by the lanes that write it, and by no others
     if (!same_view(in, out) && views_overlap(in, ib, out, ob)) return SIXI_E_INVALID_ARGUMENT;
     t->in = static_cast<const char*>(in.data);
@@ -80,7 +80,7 @@ int resolve(const sixi_qk_rope_params* p, sixi::RopeArgs* out) {
             return SIXI_E_INVALID_ARGUMENT;
     }
     if (D <= 0 || D % 16 != 0 || D > 256) return SIXI_E_UNSUPPORTED;
-    if (S > 65535) return SIXI_E_UNSUPPORTED;
+    if (S > 65535 || n_rows > (1 << 23) || p->q.ne[1] > 65535 || (has_k && p->k.ne[1] > 65535)) return SIXI_E_UNSUPPORTED;
     if (p->n_rot < 0 || p->n_rot > D || p->n_rot % 16 != 0) return SIXI_E_INVALID_ARGUMENT;
     if (p->n_rot > 0 && !p->freqs) return SIXI_E_INVALID_ARGUMENT;
     if (!aligned(p->freqs, 8) || !aligned(p->kv_len, 4) || !aligned(p->pos, 4) || !aligned(p->q_len, 4)) return SIXI_E_ALIGNMENT;
@@ -91,6 +91,18 @@ int resolve(const sixi_qk_rope_params* p, sixi::RopeArgs* out) {
     if (!aligned(p->q_norm, 16) || !aligned(p->k_norm, 16)) return SIXI_E_ALIGNMENT;
     if (!std::isfinite(p->mscale)) return SIXI_E_INVALID_ARGUMENT;
     if (p->pos && p->pos_stride < 0) return SIXI_E_INVALID_ARGUMENT;
+    if (p->pos && p->pos_stride > INT32_MAX) return SIXI_E_INTEGER_OVERFLOW;
+    // rows are written while other work-groups read these
+    const struct { const void* p; int64_t bytes; } read[] = {
+        {p->freqs, (int64_t)p->n_rot / 2 * 8},  {p->q_norm, norm ? D * 4 : 0}, {p->k_norm, p->k_norm ? D * 4 : 0},
+        {p->kv_len, p->kv_len ? S * 4 : 0},     {p->q_len, p->q_len ? S * 4 : 0},
+        {p->pos, p->pos && S > 0 ? ((S - 1) * p->pos_stride + n_rows) * 4 : 0}};
+    for (int i = 0; i < (has_k ? 2 : 1); ++i) {
+        const sixi_view& w = i ? p->k_out : p->q_out;
+        const int64_t span = view_span(w, D * elem_bytes(w.type));
+        for (const auto& r : read)
+            if (ranges_overlap(w.data, span, r.p, r.bytes)) return SIXI_E_INVALID_ARGUMENT;
+    }
     a.t[0].norm = p->q_norm;
     a.t[1].norm = p->k_norm;
     a.freqs = p->freqs;

@@ -171,7 +171,7 @@ def test_exponents_out_of_range_count_as_the_nearest():
 # ---- attention ----
 
 def _attend(s, n_q, H, heads, d, cached, rows, cells, mode=sa.MASK_BLOCK_CAUSAL, paged=False, q16=True, o16=True,
-            scale=None, seed=0, mask=None, exps=(-6, -3), q_size=2.0, no_lens=False, handle=None):
+            scale=None, seed=0, mask=None, exps=(-6, -3), q_size=2.0, no_lens=False, no_rows=False, handle=None):
     _say(f"kv8 attention s={s} n_q={n_q} H={H} heads={heads} d={d} cached={cached} rows={rows} cells={cells} mode={mode} "
          f"paged={paged} q16={q16} o16={o16} scale={scale} exps={exps}")
     rng = np.random.default_rng(seed + n_q * 7 + d + sum(cached))
@@ -185,7 +185,7 @@ def _attend(s, n_q, H, heads, d, cached, rows, cells, mode=sa.MASK_BLOCK_CAUSAL,
     out = torch.full((s, n_q, H, d), float("nan"), dtype=torch.float16 if o16 else torch.float32, device="cuda")
     sc = d ** -0.5 if scale is None else scale
     fa = handle or sa.Kv8Attention()
-    fa(torch.from_numpy(q).cuda(), cache, out, kv_len=None if no_lens else _i32(cached), q_len=_i32(rows), mask_mode=mode,
+    fa(torch.from_numpy(q).cuda(), cache, out, kv_len=None if no_lens else _i32(cached), q_len=None if no_rows else _i32(rows), mask_mode=mode,
        mask=None if mask is None else torch.from_numpy(mask).cuda(), scale=scale, page_table=table)
     want, tol = attention(q.astype(np.float16).astype(np.float64), k.values(), v.values(), v.exps, cached, rows, sc, mode,
                           None if mask is None else mask.astype(np.float64))
@@ -235,6 +235,19 @@ def test_attention_pages(d, rows):
 def test_attention_long(d):
     _attend(1, 2, 6, 1, d, [20011], [2], 20480)
     _attend(2, 1, 6, 1, d, [9000, 33], [1, 1], 9216, paged=True, seed=1)
+
+
+@pytest.mark.parametrize("d", [128, 256])
+def test_attention_rows_of_every_stream(d):
+    """Without q_len the host can tell whether there is anything to join: few tiles, just enough of them, and more."""
+    for s, n_q in ((2, 20), (15, 127), (16, 128), (17, 129)):
+        _attend(s, n_q, 12, 4, d, [5 * i % 70 for i in range(s)], [n_q] * s, 256, no_rows=True)
+
+
+def test_attention_few_rows_of_a_long_block():
+    """Rows for many tiles, few of them there: their cells are cut and joined."""
+    _attend(2, 2000, 24, 4, 128, [1500, 2000], [40, 3], 4096)
+    _attend(1, 700, 8, 1, 256, [900], [90], 2048, paged=True)
 
 
 def test_attention_without_lengths_sees_every_cell():
