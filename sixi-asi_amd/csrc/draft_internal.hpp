@@ -51,9 +51,10 @@ struct DraftArgs {
     int32_t* token;
     DraftPart* parts;  // [S][n_rows][n_parts]
     DraftDraw* draws;  // [S][chunks]
-    int32_t* counts;   // [S]: work-groups that have left their share in draws
+    int32_t* counts;   // [S]: chunks whose share is in draws
     int32_t V, n_rows, S, chunks;  // chunks of a row
     int32_t run, n_parts;          // chunks that a work-group of the rows takes; such work-groups of a row
+    int32_t draw_run;              // chunks that a work-group of the draw takes
 };
 
 hipError_t launch_draft_verify(const DraftArgs& a, hipStream_t stream);

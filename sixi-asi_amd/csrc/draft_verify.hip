@@ -443,7 +443,7 @@ __device__ __forceinline__ DraftFound find_chunk(const DraftArgs& a, int s, doub
     return f;
 }
 
-// A stream's chunks; the last work-group goes through the chunk found once more.
+// A stream's chunks, a.draw_run to a work-group; the last work-group goes through the chunk found once more.
 template <int TYPE>
 __global__ __launch_bounds__(kThreads) void draft_draw_kernel(DraftArgs a) {
     __shared__ double ws[kThreads / 64], ps[kThreads / 64];
@@ -461,14 +461,16 @@ __global__ __launch_bounds__(kThreads) void draft_draw_kernel(DraftArgs a) {
     const double u_next = (double)a.u_next[s];
     const DraftVerdict v = decide(a, s, rows, sums, &stop);
     if (blockIdx.x == 0 && tid == 0) a.keep[s] = v.row + 1;
-    DraftFound f{0.0, 0.0, (int)blockIdx.x, -1, true};
+    const int first = blockIdx.x * a.draw_run, end = min(first + a.draw_run, a.chunks);
+    DraftFound f{0.0, 0.0, first, -1, true};
+    bool found = false;
 #pragma unroll 1
-    for (int pass = 0;; ++pass) {
+    while (true) {
         // 16 consecutive tokens per thread
         double w[kPer], p[kPer];
         const int t0 = f.chunk * kDraftChunk + tid * kPer;
         weights_of<TYPE>(a, s, v, t0, w, p);
-        if (pass == 0) {
+        if (!found) {
             double sum_w = 0.0, sum_p = 0.0;
             int last_w = -1, last_p = -1;
 #pragma unroll
@@ -493,12 +495,16 @@ __global__ __launch_bounds__(kThreads) void draft_draw_kernel(DraftArgs a) {
                 put(a.draws + (int64_t)s * a.chunks + f.chunk,
                     {((ws[0] + ws[1]) + ws[2]) + ws[3], ((ps[0] + ps[1]) + ps[2]) + ps[3], max(max(lws[0], lws[1]), max(lws[2], lws[3])),
                      max(max(lps[0], lps[1]), max(lps[2], lps[3]))});
-                // counted once the stores above have reached the device's memory
-                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                last = __hip_atomic_fetch_add(a.counts + s, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+                if (f.chunk + 1 == end) {
+                    // counted once the stores above have reached the device's memory
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    last = __hip_atomic_fetch_add(a.counts + s, end - first, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + end - first == a.chunks;
+                }
             }
             __syncthreads();
+            if (++f.chunk < end) continue;
             if (!last) return;
+            found = true;
             f = find_chunk(a, s, u_next);
             if (f.chunk < 0) {
                 if (tid == 0) a.token[s] = -1;
@@ -522,18 +528,18 @@ __global__ __launch_bounds__(kThreads) void draft_draw_kernel(DraftArgs a) {
         if (stop == kThreads) {  // (the chunk's end is past the mark by less than its sums' rounding)
             if (tid == 0) a.token[s] = f.last;
         } else if (tid == stop) {
-            int found = -1;
+            int token = -1;
             bool done = false;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const double x = f.from_w ? w[i] : p[i];
                 if (!done && x > 0.0) {
                     at += x;
-                    found = t0 + i;
+                    token = t0 + i;
                     done = at > f.mark;
                 }
             }
-            a.token[s] = found;
+            a.token[s] = token;
         }
         return;
     }
@@ -544,7 +550,7 @@ hipError_t launch(const DraftArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL(draft_rows_kernel<TYPE>, dim3((unsigned)a.n_parts, (unsigned)a.n_rows, (unsigned)a.S), dim3(kThreads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(draft_draw_kernel<TYPE>, dim3((unsigned)a.chunks, (unsigned)a.S), dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(draft_draw_kernel<TYPE>, dim3((unsigned)((a.chunks + a.draw_run - 1) / a.draw_run), (unsigned)a.S), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
 

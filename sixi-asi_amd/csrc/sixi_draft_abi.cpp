@@ -5,6 +5,7 @@
 // include/sixi_asi/common.hpp:40-67, negated).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "abi_util.hpp"
@@ -98,6 +99,10 @@ int resolve(const sixi_draft_params* p, sixi::DraftArgs* out, size_t* ws) {
     // four chunks in a row where one each would be more than four work-groups for each of 8 places of a CU
     a.run = S * rows * a.chunks > 4 * 8 * (int64_t)sixi::device_cu_count() ? 4 : 1;
     a.n_parts = (a.chunks + a.run - 1) / a.run;
+    // a work-group of the draw first forms the accept chain again: no more of them than run at once, 3 on a CU
+    // (32 streams of 61 chunks: 25 us, with a chunk each 29)
+    const int64_t places = 3 * (int64_t)sixi::device_cu_count();
+    a.draw_run = (int32_t)std::clamp<int64_t>((S * a.chunks + places - 1) / places, 1, 8);
     const int64_t parts = S * rows * a.n_parts * (int64_t)sizeof(sixi::DraftPart);  // < 2^16 * 2^10 * 2^18 * 2^4
     const int64_t draws = S * a.chunks * (int64_t)sizeof(sixi::DraftDraw);
     *ws = (size_t)(parts + draws) + (size_t)S * sizeof(int32_t);
