@@ -11,16 +11,17 @@
 //   O' = sum P' v,   l = sum P' 2^-ev,   o = O' / l
 // With ev inside the exponent a block's V scale costs nothing, and the f16 rounding of P' is half a step
 // of 11 bits of each weight, down to 2^-24 of the largest contribution whatever the blocks' scales are.
-// l is the f32 sum of the same f16 weights.
+// l is the f32 sum of the weights in front of that rounding: a block with a small V scale stands next to
+// one with a large one, and its f16 weights would be too coarse for the sum they are most of.
 //
 // The cell that score register i of a lane holds is ours to choose (any order of K's rows will do):
 // lane (n, h) of the 32 x 32 result holds cells 16h .. 16h + 15 of the block in order, which is what the
 // lane needs as its half of the next product's right operand.  So P never leaves its lane.
 //
-// Two kernels.  Up to 32 rows a group (decode): the four waves of a work-group take blocks in turn,
-// straight from memory into registers, one block ahead; nothing is shared.  More rows: NW waves take 32
-// rows each of the same cells; a step's codes are converted once, by all of them, into f16 operands in
-// LDS (two buffers, the next step's codes on their way in registers).
+// Two kernels.  Up to 32 rows a group (decode), or 64 of 128 dims: the four waves of a work-group take blocks
+// in turn, straight from memory into registers, one block ahead; nothing is shared but two tiles' queries.
+// More rows: NW waves take 32 rows each of the same cells; a step's codes are converted once, by all of them,
+// into f16 operands in LDS (two buffers, the next step's codes on their way in registers).
 //
 // Work-groups: every stream's cells are cut into pieces of c blocks, c from the lengths on the device, so
 // that streams of any lengths fill the chip; pieces of one (stream, head, tile) are joined by a second
@@ -182,11 +183,10 @@ __device__ __forceinline__ void store4(const Kv8AttnArgs& a, char* row, int d, k
     }
 }
 
-// What a wave holds: 32 rows of a group, their queries and sums.
+// What a wave holds of 32 rows of a group: their sums.
 template <int D>
 struct Rows {
     static constexpr int KC = D / 32;  // 32-dim pieces of a row: K loads, V loads and output tiles
-    kv8_f16x8 q[KC][2];
     f32x16 o[KC];
     float m, l;
     int last;     // the last cell that the lane's row sees
@@ -196,7 +196,7 @@ struct Rows {
     bool live;
 
     __device__ __forceinline__ void begin(const Kv8AttnArgs& a, const Lens& n, int s, int g, int r0) {
-        const int lane = threadIdx.x & 63, M = n.rows * a.G, r = r0 + (lane & 31), h = lane >> 5;
+        const int M = n.rows * a.G, r = r0 + (threadIdx.x & 31);
         live = r < M;
         j = live ? r / a.G : 0;
         head = live ? g * a.G + r % a.G : g * a.G;
@@ -205,6 +205,15 @@ struct Rows {
         sees = causal ? n.cached + r0 / a.G : n.cells - 1;
         reach = causal ? n.cached + (min(r0 + 32, M) - 1) / a.G + 1 : n.cells;
         if (r0 >= M) reach = 0;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) o[c] = f32x16{};
+        m = kLowest;
+        l = 0.0f;
+    }
+
+    // The rows' queries as the products' right operands.
+    __device__ __forceinline__ void queries(const Kv8AttnArgs& a, int s, kv8_f16x8 (&q)[KC][2]) const {
+        const int h = (threadIdx.x & 63) >> 5;
         const char* p = a.q + (int64_t)j * a.q_nb1 + (int64_t)head * a.q_nb2 + (int64_t)s * a.q_nb3;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
@@ -228,10 +237,6 @@ struct Rows {
                 }
                 q[c][u] = x;
             }
-#pragma unroll
-        for (int c = 0; c < KC; ++c) o[c] = f32x16{};
-        m = kLowest;
-        l = 0.0f;
     }
 
     // A block's scores: hidden cells to -inf; with a mask, to t itself.
@@ -271,22 +276,10 @@ struct Rows {
         top = max_halves(__builtin_elementwise_maximum(top, top2));
         return MASK ? top : fmaf(top, ks, es);
     }
-    // A new reference where a maximum has outgrown the old one (a NaN has not; its weights are NaN).
-    __device__ __forceinline__ void raise(float top) {
-        const bool grow = top > m + kRoof;
-        if (__builtin_amdgcn_ballot_w64(grow)) {
-            const float up = grow ? top - kHead : m, f = __builtin_amdgcn_exp2f(m - up);
-            m = up;
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < KC; ++c) o[c] *= f;
-        }
-    }
     // Scores to weights in f16, and their sum.
     template <bool MASK>
     __device__ __forceinline__ void weights(const f32x16& sc, float ks, float es, int ev, kv8_f16x8 (&p)[2]) {
         const float sub = MASK ? -m : es - m;
-        const f16x2 one = {(_Float16)1.0f, (_Float16)1.0f};
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
@@ -296,7 +289,8 @@ struct Rows {
             const f16x2 x = __builtin_convertvector(w, f16x2);
             p[i / 8][i % 8] = x[0];
             p[i / 8][i % 8 + 1] = x[1];
-            sum[i / 2 % 2] = __builtin_amdgcn_fdot2(x, one, sum[i / 2 % 2], false);
+            sum[0] += w[0];
+            sum[1] += w[1];
         }
         l = fmaf(sum[0] + sum[1], exp2_int(-ev), l);
     }
@@ -329,6 +323,23 @@ struct Rows {
     }
 };
 
+// A new reference where a maximum has outgrown the old one (a NaN has not; its weights are NaN).
+template <int D, int T>
+__device__ __forceinline__ void raise(Rows<D> (&r)[T], const float (&top)[T]) {
+    bool grow = false;
+#pragma unroll
+    for (int t = 0; t < T; ++t) grow |= top[t] > r[t].m + kRoof;
+    if (!__builtin_amdgcn_ballot_w64(grow)) return;
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        const float up = top[t] > r[t].m + kRoof ? top[t] - kHead : r[t].m, f = __builtin_amdgcn_exp2f(r[t].m - up);
+        r[t].m = up;
+        r[t].l *= f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) r[t].o[c] *= f;
+    }
+}
+
 // The piece of a work-group, in the order (stream, tile from the last on, piece, head): the longest tiles of a
 // causal chunk first, and, as work-groups go round the 8 XCDs, tiles of the same head on few of them, where
 // they meet in the L2.
@@ -357,7 +368,7 @@ __device__ __forceinline__ bool work_of(const Kv8AttnArgs& a, Work& w) {
 
 constexpr int kWaves = 4;
 
-template <int D, bool MASK>
+template <int D, int T, bool MASK>
 __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_kernel(Kv8AttnArgs a) {
     constexpr int KC = D / 32;
     extern __shared__ __align__(16) float lds[];
@@ -367,8 +378,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
     if (!work_of(a, w)) return;
     // cells that any row sees
     int last = w.last;
+    const int r0 = w.tile * (32 * T);
     if (a.mode == SIXI_MASK_BLOCK_CAUSAL)
-        last = min(last, (w.n.cached + (min(w.tile * 32 + 32, w.n.rows * a.G) - 1) / a.G + kBlk) / kBlk);
+        last = min(last, (w.n.cached + (min(r0 + 32 * T, w.n.rows * a.G) - 1) / a.G + kBlk) / kBlk);
     const uint32_t k_off = h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
     const uint32_t v_off = n * kBlk + h * 16;
 
@@ -387,13 +399,37 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
 #pragma unroll
         for (int c = 0; c < KC; ++c) vc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.v + v_off + c * (kBlk * 32));
     }
-    Rows<D> r;
-    r.begin(a, w.n, w.s, w.g, w.tile * 32);
-    const char* mask = MASK ? a.mask + (int64_t)r.j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
+    Rows<D> r[T];
+    const char* mask[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        r[t].begin(a, w.n, w.s, w.g, r0 + t * 32);
+        mask[t] = MASK ? a.mask + (int64_t)r[t].j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
+    }
+    kv8_f16x8 q[KC][2];
+    // several tiles' queries stay in LDS, for all waves: [tile][piece][first, second eight][lane]
+    typedef kv8_f16x8 Queries[KC][2][64];
+    Queries* qs = reinterpret_cast<Queries*>(lds);
+    if constexpr (T == 1) {
+        r[0].queries(a, w.s, q);
+    } else {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+            if (wave == t) {
+                r[t].queries(a, w.s, q);
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) qs[t][c][u][lane] = q[c][u];
+            }
+        __syncthreads();
+    }
     if (b < last) {
         walk.go(a.pages, a.k, a.v, w.s, w.g, kWaves);
         for (; b < last; b += kWaves) {
-            f32x16 sc = {};
+            f32x16 sc[T] = {};
+            int at = lane;  // (read from LDS in every step: out of the loop they would fill the registers)
+            if (T > 1) asm volatile("" : "+v"(at));
             kv8_f16x8 x[KC][2];
 #pragma unroll
             for (int c = 0; c < KC; ++c) codes_f16x16(kc[c], x[c][0], x[c][1]);
@@ -405,59 +441,86 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
             const char* vn = walk.v;
             walk.go(a.pages, a.k, a.v, w.s, w.g, kWaves);
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                sc = mfma(x[c][0], r.q[c][0], sc);
-                sc = mfma(x[c][1], r.q[c][1], sc);
-            }
-            kv8_f16x8 p[2];
-            const float ks = a.scale_log2 * exp2_int(ek0), es = (float)ev0;
-            r.template hide<MASK>(a, sc, b, ks, es, mask);
-            r.raise(r.template top_of<MASK>(sc, ks, es));
-            r.template weights<MASK>(sc, ks, es, ev0, p);
+            for (int c = 0; c < KC; ++c)
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                kv8_f16x8 y[2];
-                codes_f16x16(vc[c], y[0], y[1]);
-                vc[c] = *reinterpret_cast<const kv8_u32x4*>(vn + v_off + c * (kBlk * 32));
-                r.o[c] = mfma(y[0], p[0], r.o[c]);
-                r.o[c] = mfma(y[1], p[1], r.o[c]);
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int t = 0; t < T; ++t) sc[t] = mfma(x[c][u], T == 1 ? q[c][u] : qs[t][c][u][at], sc[t]);
+            const float ks = a.scale_log2 * exp2_int(ek0), es = (float)ev0;
+            float top[T];
+#pragma unroll
+            for (int t = 0; t < T; ++t) {
+                r[t].template hide<MASK>(a, sc[t], b, ks, es, mask[t]);
+                top[t] = r[t].template top_of<MASK>(sc[t], ks, es);
+            }
+            raise(r, top);
+            if constexpr (T == 1) {
+                kv8_f16x8 p[2];
+                r[0].template weights<MASK>(sc[0], ks, es, ev0, p);
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    kv8_f16x8 y[2];
+                    codes_f16x16(vc[c], y[0], y[1]);
+                    vc[c] = *reinterpret_cast<const kv8_u32x4*>(vn + v_off + c * (kBlk * 32));
+                    r[0].o[c] = mfma(y[0], p[0], r[0].o[c]);
+                    r[0].o[c] = mfma(y[1], p[1], r[0].o[c]);
+                }
+            } else {
+                kv8_f16x8 y[KC][2];
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    codes_f16x16(vc[c], y[c][0], y[c][1]);
+                    vc[c] = *reinterpret_cast<const kv8_u32x4*>(vn + v_off + c * (kBlk * 32));
+                }
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    kv8_f16x8 p[2];
+                    r[t].template weights<MASK>(sc[t], ks, es, ev0, p);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int c = 0; c < KC; ++c) r[t].o[c] = mfma(y[c][u], p[u], r[t].o[c]);
+                }
             }
         }
     }
-    r.l = sum_halves(r.l);
-
-    // the waves' results into LDS, and a quarter of the accumulators out of it for each wave
-    r.leave(lds + wave * tile_floats(D));
-    __syncthreads();
-    if (!r.live) return;
-    float m = kLowest, l = 0.0f, f[kWaves];
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-        f[k] = lds[k * tile_floats(D) + 32 * D + n];
-        m = fmaxf(m, f[k]);
-    }
+    for (int t = 0; t < T; ++t) {
+        r[t].l = sum_halves(r[t].l);
+        // the waves' results into LDS, and a quarter of the accumulators out of it for each wave
+        if (T > 1) __syncthreads();
+        r[t].leave(lds + wave * tile_floats(D));
+        __syncthreads();
+        if (!r[t].live) continue;
+        float m = kLowest, l = 0.0f, f[kWaves];
 #pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-        f[k] = __builtin_amdgcn_exp2f(f[k] - m);
-        l = fmaf(lds[k * tile_floats(D) + 32 * D + 32 + n], f[k], l);
-    }
-    const float inv = w.pieces > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
-    char* row = a.out + (int64_t)r.head * a.o_nb1 + (int64_t)r.j * a.o_nb2 + (int64_t)w.s * a.o_nb3;
-    float* part = a.part + w.id * tile_floats(D);
+        for (int k = 0; k < kWaves; ++k) {
+            f[k] = lds[k * tile_floats(D) + 32 * D + n];
+            m = fmaxf(m, f[k]);
+        }
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-        const int quad = wave * (D / 32) + i;
-        kv8_f32x4 x = {};
+        for (int k = 0; k < kWaves; ++k) {
+            f[k] = __builtin_amdgcn_exp2f(f[k] - m);
+            l = fmaf(lds[k * tile_floats(D) + 32 * D + 32 + n], f[k], l);
+        }
+        const float inv = w.pieces > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+        char* row = a.out + (int64_t)r[t].head * a.o_nb1 + (int64_t)r[t].j * a.o_nb2 + (int64_t)w.s * a.o_nb3;
+        float* part = a.part + ((int64_t)w.id * T + t) * tile_floats(D);
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) x += *reinterpret_cast<const kv8_f32x4*>(lds + k * tile_floats(D) + (quad * 64 + lane) * 4) * f[k];
-        if (w.pieces > 1)
-            *reinterpret_cast<kv8_f32x4*>(part + (quad * 64 + lane) * 4) = x;
-        else
-            store4(a, row, quad / 4 * 32 + quad % 4 * 8 + 4 * h, x * inv);
-    }
-    if (w.pieces > 1 && wave == 0 && h == 0) {
-        part[32 * D + n] = m;
-        part[32 * D + 32 + n] = l;
+        for (int i = 0; i < D / 32; ++i) {
+            const int quad = wave * (D / 32) + i;
+            kv8_f32x4 x = {};
+#pragma unroll
+            for (int k = 0; k < kWaves; ++k) x += *reinterpret_cast<const kv8_f32x4*>(lds + k * tile_floats(D) + (quad * 64 + lane) * 4) * f[k];
+            if (w.pieces > 1)
+                *reinterpret_cast<kv8_f32x4*>(part + (quad * 64 + lane) * 4) = x;
+            else
+                store4(a, row, quad / 4 * 32 + quad % 4 * 8 + 4 * h, x * inv);
+        }
+        if (w.pieces > 1 && wave == 0 && h == 0) {
+            part[32 * D + n] = m;
+            part[32 * D + 32 + n] = l;
+        }
     }
 }
 
@@ -495,8 +558,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
     Work w;
     if (!work_of(a, w)) return;
     const int r0 = w.tile * (32 * NW);
-    Rows<D> r;
+    Rows<D> one[1], &r = one[0];
     r.begin(a, w.n, w.s, w.g, r0 + wave * 32);
+    kv8_f16x8 q[KC][2];
+    r.queries(a, w.s, q);
     const char* mask = MASK ? a.mask + (int64_t)r.j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
     int last = w.last;  // blocks that any row of the work-group sees
     if (a.mode == SIXI_MASK_BLOCK_CAUSAL)
@@ -575,7 +640,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int i = 0; i < NB; ++i) sc[i] = mfma(tile[buf][0][i * KC + c][u][lane], r.q[c][u], sc[i]);
+                        for (int i = 0; i < NB; ++i) sc[i] = mfma(tile[buf][0][i * KC + c][u][lane], q[c][u], sc[i]);
                 feed<2 * NB * KC, kAhead>();
                 __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
@@ -588,13 +653,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
             }
             if (any) {
                 kv8_f16x8 p[NB][2];
-                float top = kLowest;
+                float top[1] = {kLowest};
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
                     r.template hide<MASK>(a, sc[i], b + i, ks[i], es[i], mask);
-                    top = __builtin_elementwise_maximum(top, r.template top_of<MASK>(sc[i], ks[i], es[i]));
+                    top[0] = __builtin_elementwise_maximum(top[0], r.template top_of<MASK>(sc[i], ks[i], es[i]));
                 }
-                r.raise(top);
+                raise(one, top);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) r.template weights<MASK>(sc[i], ks[i], es[i], e0[i], p[i]);
                 __builtin_amdgcn_sched_barrier(0);
@@ -732,16 +797,19 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a) {
     store4(a, a.out + (int64_t)head * a.o_nb1 + (int64_t)j * a.o_nb2 + (int64_t)s * a.o_nb3, quad / 4 * 32 + quad % 4 * 8 + 4 * h, o * inv);
 }
 
+template <int D, int T, bool MASK>
+void launch_few(const Kv8AttnArgs& a, hipStream_t stream) {
+    const size_t lds = (size_t)kWaves * tile_floats(D) * sizeof(float);
+    hipLaunchKernelGGL((kv8_attn_few_kernel<D, T, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
+}
 template <int D, bool MASK>
 void launch_pieces(const Kv8AttnArgs& a, hipStream_t stream) {
-    if (a.waves == 1) {
-        const size_t lds = (size_t)kWaves * tile_floats(D) * sizeof(float);
-        hipLaunchKernelGGL((kv8_attn_few_kernel<D, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
-    } else {
-        constexpr int NB = D == 128 ? 2 : 1;
-        constexpr size_t lds = rows_lds<D, NB>();
-        hipLaunchKernelGGL((kv8_attn_rows_kernel<D, NB, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
-    }
+    if (a.waves == 1) return launch_few<D, 1, MASK>(a, stream);
+    if constexpr (D == 128 && !MASK)
+        if (a.waves == 2) return launch_few<D, 2, MASK>(a, stream);
+    constexpr int NB = D == 128 ? 2 : 1;
+    constexpr size_t lds = rows_lds<D, NB>();
+    hipLaunchKernelGGL((kv8_attn_rows_kernel<D, NB, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
 }
 
 template <int D>
@@ -762,7 +830,11 @@ hipError_t launch(const Kv8AttnArgs& a, hipStream_t stream) {
 
 size_t kv8_attn_plan(Kv8AttnArgs& a) {
     const int64_t t32 = ((int64_t)a.n_q * a.G + 31) / 32;
-    a.waves = t32 == 1 ? 1 : kWaves;
+    // 33 to 64 rows of 128 dims: both tiles in every wave's registers, where two of the rows kernel's four waves
+    // would only convert (32 streams of 48 rows, up to 16k cells: 75 against 95 us).  Not with a mask: its values
+    // do not fit beside them (32 streams of 60 rows: 175 against 118 us).
+    const bool two = t32 == 2 && a.D == 128 && a.mode != SIXI_MASK_EXPLICIT;
+    a.waves = t32 == 1 ? 1 : two ? 2 : kWaves;
     a.target = 2 * device_cu_count();
     a.least = 4;
     const int64_t tiles = (t32 + a.waves - 1) / a.waves * a.Hkv * a.S;

@@ -244,6 +244,22 @@ def test_attention_rows_of_every_stream(d):
         _attend(s, n_q, 12, 4, d, [5 * i % 70 for i in range(s)], [n_q] * s, 256, no_rows=True)
 
 
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("n_q,H,heads", [(6, 24, 4), (8, 24, 4), (11, 24, 4), (16, 24, 4), (64, 2, 2), (90, 1, 1), (3, 32, 1)])
+def test_attention_of_33_to_96_rows(d, n_q, H, heads):
+    """Two and three tiles of rows in one work-group: lengths about its steps of 128 cells and their pieces, ragged rows,
+    pages, and scales that outgrow the reference again and again."""
+    for i, cached in enumerate([[0, 1, 90], [127, 128, 129], [255, 700, 1023 - n_q], [1500, 0, 5]]):
+        rows = [n_q, max(1, n_q // 2), n_q if i % 2 else 0]
+        _attend(3, n_q, H, heads, d, cached, rows, 1792, paged=i % 2 == 1, q16=i < 2, o16=i > 0, seed=i)
+        _attend(3, n_q, H, heads, d, cached, rows, 1792, exps=(-16, 8), q_size=0.05, mode=sa.MASK_NONE if i == 3 else sa.MASK_BLOCK_CAUSAL,
+                seed=10 + i)
+    rng = np.random.default_rng(n_q)
+    for hidden in (-np.inf, -65504.0):
+        m = _tree(rng, 2, n_q, 1024, [800, 90], [n_q, n_q], hidden)
+        _attend(2, n_q, H, heads, d, [800, 90], [n_q, n_q], 1024, mode=sa.MASK_EXPLICIT, mask=m, seed=5)
+
+
 def test_attention_few_rows_of_a_long_block():
     """Rows for many tiles, few of them there: their cells are cut and joined."""
     _attend(2, 2000, 24, 4, 128, [1500, 2000], [40, 3], 4096)
