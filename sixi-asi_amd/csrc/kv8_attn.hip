@@ -239,26 +239,21 @@ struct Rows {
             }
     }
 
+    // The mask's values for the lane's 16 cells of a block (all of a block's are there, whatever the row sees).
+    __device__ __forceinline__ static void mask_of(const char* mask, int block, f16x8u (&add)[2]) {
+        const char* p = mask + (int64_t)(block * kBlk + 16 * ((threadIdx.x & 63) >> 5)) * 2;
+        add[0] = *reinterpret_cast<const f16x8u*>(p);
+        add[1] = *reinterpret_cast<const f16x8u*>(p + 16);
+    }
     // A block's scores: hidden cells to -inf; with a mask, to t itself.
     template <bool MASK>
-    __device__ __forceinline__ void hide(const Kv8AttnArgs& a, f32x16& sc, int block, float ks, float es, const char* mask) const {
+    __device__ __forceinline__ void hide(f32x16& sc, int block, float ks, float es, const f16x8u (&add)[2]) const {
         const int cell0 = block * kBlk + 16 * ((threadIdx.x & 63) >> 5);
         if (MASK) {
-            f16x8u add[2];
-            if (block * kBlk + kBlk - 1 <= last) {
-                add[0] = *reinterpret_cast<const f16x8u*>(mask + (int64_t)cell0 * 2);
-                add[1] = *reinterpret_cast<const f16x8u*>(mask + (int64_t)cell0 * 2 + 16);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    _Float16 x = (_Float16)-__builtin_huge_valf();
-                    if (cell0 + i <= last) x = *reinterpret_cast<const _Float16*>(mask + (int64_t)(cell0 + i) * 2);
-                    add[i / 8][i % 8] = x;
-                }
-            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[i] = fmaf(sc[i], ks, fmaf((float)add[i / 8][i % 8], kLog2e, es));
-        } else if (block * kBlk + kBlk - 1 > sees) {
+        }
+        if (block * kBlk + kBlk - 1 > sees) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 if (cell0 + i > last) sc[i] = -__builtin_huge_valf();
@@ -425,6 +420,10 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
         __syncthreads();
     }
     if (b < last) {
+        f16x8u add[T][2], next[T][2];
+        if (MASK)
+#pragma unroll
+            for (int t = 0; t < T; ++t) Rows<D>::mask_of(mask[t], b, next[t]);
         walk.go(a.pages, a.k, a.v, w.s, w.g, kWaves);
         for (; b < last; b += kWaves) {
             f32x16 sc[T] = {};
@@ -438,6 +437,13 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
             for (int c = 0; c < KC; ++c) kc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.k + k_off + c * (kBlk * 32));
             ek = *walk.ke;
             ev = *walk.ve;
+            if (MASK)
+#pragma unroll
+                for (int t = 0; t < T; ++t) {
+                    add[t][0] = next[t][0];
+                    add[t][1] = next[t][1];
+                    Rows<D>::mask_of(mask[t], walk.b, next[t]);
+                }
             const char* vn = walk.v;
             walk.go(a.pages, a.k, a.v, w.s, w.g, kWaves);
 #pragma unroll
@@ -450,7 +456,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
             float top[T];
 #pragma unroll
             for (int t = 0; t < T; ++t) {
-                r[t].template hide<MASK>(a, sc[t], b, ks, es, mask[t]);
+                r[t].template hide<MASK>(sc[t], b, ks, es, add[t]);
                 top[t] = r[t].template top_of<MASK>(sc[t], ks, es);
             }
             raise(r, top);
@@ -632,7 +638,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                 load_exps();
                 walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
             }
+            f16x8u add[NB][2];
             if (any) {
+                if (MASK)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) Rows<D>::mask_of(mask, min(b + i, last - 1), add[i]);
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -656,7 +666,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                 float top[1] = {kLowest};
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
-                    r.template hide<MASK>(a, sc[i], b + i, ks[i], es[i], mask);
+                    r.template hide<MASK>(sc[i], b + i, ks[i], es[i], add[i]);
                     top[0] = __builtin_elementwise_maximum(top[0], r.template top_of<MASK>(sc[i], ks[i], es[i]));
                 }
                 raise(one, top);
