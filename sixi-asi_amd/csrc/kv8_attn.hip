@@ -183,6 +183,17 @@ __device__ __forceinline__ void store4(const Kv8AttnArgs& a, char* row, int d, k
     }
 }
 
+// Which row of a group's 32 is the lane's: row j of the block, q-head `head`.
+struct Seat {
+    int j, head;
+    bool live;
+};
+__device__ __forceinline__ Seat seat_of(const Kv8AttnArgs& a, const Lens& n, int g, int r0) {
+    const int r = r0 + (threadIdx.x & 31);
+    const bool live = r < n.rows * a.G;
+    return {live ? r / a.G : 0, g * a.G + (live ? r % a.G : 0), live};
+}
+
 // What a wave holds of 32 rows of a group: their sums.
 template <int D>
 struct Rows {
@@ -192,16 +203,11 @@ struct Rows {
     int last;     // the last cell that the lane's row sees
     int sees;     // the last cell that every row sees
     int reach;    // cells that any of the rows sees
-    int j, head;
-    bool live;
 
-    __device__ __forceinline__ void begin(const Kv8AttnArgs& a, const Lens& n, int s, int g, int r0) {
-        const int M = n.rows * a.G, r = r0 + (threadIdx.x & 31);
-        live = r < M;
-        j = live ? r / a.G : 0;
-        head = live ? g * a.G + r % a.G : g * a.G;
+    __device__ __forceinline__ void begin(const Kv8AttnArgs& a, const Lens& n, int r0, const Seat& x) {
+        const int M = n.rows * a.G;
         const bool causal = a.mode == SIXI_MASK_BLOCK_CAUSAL;
-        last = causal ? n.cached + j : n.cells - 1;
+        last = causal ? n.cached + x.j : n.cells - 1;
         sees = causal ? n.cached + r0 / a.G : n.cells - 1;
         reach = causal ? n.cached + (min(r0 + 32, M) - 1) / a.G + 1 : n.cells;
         if (r0 >= M) reach = 0;
@@ -212,16 +218,16 @@ struct Rows {
     }
 
     // The rows' queries as the products' right operands.
-    __device__ __forceinline__ void queries(const Kv8AttnArgs& a, int s, kv8_f16x8 (&q)[KC][2]) const {
+    __device__ __forceinline__ static void queries(const Kv8AttnArgs& a, int s, const Seat& seat, kv8_f16x8 (&q)[KC][2]) {
         const int h = (threadIdx.x & 63) >> 5;
-        const char* p = a.q + (int64_t)j * a.q_nb1 + (int64_t)head * a.q_nb2 + (int64_t)s * a.q_nb3;
+        const char* p = a.q + (int64_t)seat.j * a.q_nb1 + (int64_t)seat.head * a.q_nb2 + (int64_t)s * a.q_nb3;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int d = (2 * c + h) * 16 + 8 * u;
                 kv8_f16x8 x = {};
-                if (live) {
+                if (seat.live) {
                     if (a.q_f16) {
                         x = *reinterpret_cast<const kv8_f16x8*>(p + d * 2);
                     } else {
@@ -290,11 +296,11 @@ struct Rows {
         l = fmaf(sum[0] + sum[1], exp2_int(-ev), l);
     }
 
-    __device__ __forceinline__ void finish(const Kv8AttnArgs& a, int s) {
-        if (!live) return;
+    __device__ __forceinline__ void finish(const Kv8AttnArgs& a, int s, const Seat& seat) const {
+        if (!seat.live) return;
         const int h = (threadIdx.x & 63) >> 5;
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-        char* row = a.out + (int64_t)head * a.o_nb1 + (int64_t)j * a.o_nb2 + (int64_t)s * a.o_nb3;
+        char* row = a.out + (int64_t)seat.head * a.o_nb1 + (int64_t)seat.j * a.o_nb2 + (int64_t)s * a.o_nb3;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -302,9 +308,9 @@ struct Rows {
                 store4(a, row, c * 32 + 2 * i + 4 * h, kv8_f32x4{o[c][i], o[c][i + 1], o[c][i + 2], o[c][i + 3]} * inv);
     }
 
-    __device__ __forceinline__ void leave(float* part) {
+    __device__ __forceinline__ void leave(float* part, const Seat& seat) const {
         const int lane = threadIdx.x & 63;
-        if (!live) return;
+        if (!seat.live) return;
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -395,23 +401,25 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
         for (int c = 0; c < KC; ++c) vc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.v + v_off + c * (kBlk * 32));
     }
     Rows<D> r[T];
+    Seat seat[T];
     const char* mask[T];
 #pragma unroll
     for (int t = 0; t < T; ++t) {
-        r[t].begin(a, w.n, w.s, w.g, r0 + t * 32);
-        mask[t] = MASK ? a.mask + (int64_t)r[t].j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
+        seat[t] = seat_of(a, w.n, w.g, r0 + t * 32);
+        r[t].begin(a, w.n, r0 + t * 32, seat[t]);
+        mask[t] = MASK ? a.mask + (int64_t)seat[t].j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
     }
     kv8_f16x8 q[KC][2];
     // several tiles' queries stay in LDS, for all waves: [tile][piece][first, second eight][lane]
     typedef kv8_f16x8 Queries[KC][2][64];
     Queries* qs = reinterpret_cast<Queries*>(lds);
     if constexpr (T == 1) {
-        r[0].queries(a, w.s, q);
+        Rows<D>::queries(a, w.s, seat[0], q);
     } else {
 #pragma unroll
         for (int t = 0; t < T; ++t)
             if (wave == t) {
-                r[t].queries(a, w.s, q);
+                Rows<D>::queries(a, w.s, seat[t], q);
 #pragma unroll
                 for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -495,9 +503,9 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
         r[t].l = sum_halves(r[t].l);
         // the waves' results into LDS, and a quarter of the accumulators out of it for each wave
         if (T > 1) __syncthreads();
-        r[t].leave(lds + wave * tile_floats(D));
+        r[t].leave(lds + wave * tile_floats(D), seat[t]);
         __syncthreads();
-        if (!r[t].live) continue;
+        if (!seat[t].live) continue;
         float m = kLowest, l = 0.0f, f[kWaves];
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
@@ -510,7 +518,7 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
             l = fmaf(lds[k * tile_floats(D) + 32 * D + 32 + n], f[k], l);
         }
         const float inv = w.pieces > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
-        char* row = a.out + (int64_t)r[t].head * a.o_nb1 + (int64_t)r[t].j * a.o_nb2 + (int64_t)w.s * a.o_nb3;
+        char* row = a.out + (int64_t)seat[t].head * a.o_nb1 + (int64_t)seat[t].j * a.o_nb2 + (int64_t)w.s * a.o_nb3;
         float* part = a.part + ((int64_t)w.id * T + t) * tile_floats(D);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
@@ -553,28 +561,29 @@ template <int D, int NB, bool MASK>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnArgs a) {
     constexpr int NW = kWaves;
     constexpr int KC = D / 32, ITEMS = NB * KC, MINE = ITEMS / NW;
-    constexpr int kAhead = D == 128 ? 6 : 4;  // LDS reads ahead of their products
+    constexpr int kAhead = D == 128 ? 6 : 3;  // LDS reads ahead of their products
     static_assert(ITEMS % NW == 0, "every wave converts the same share");
     extern __shared__ __align__(16) float lds[];
     // [buffer][K, V][block, piece][first, second eight][lane] 8 f16
     typedef kv8_f16x8 Tile[2][ITEMS][2][64];
     Tile* tile = reinterpret_cast<Tile*>(lds);
-    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     Work w;
     if (!work_of(a, w)) return;
     const int r0 = w.tile * (32 * NW);
+    int mine = r0 + wave * 32;
+    Seat seat = seat_of(a, w.n, w.g, mine);
     Rows<D> one[1], &r = one[0];
-    r.begin(a, w.n, w.s, w.g, r0 + wave * 32);
+    r.begin(a, w.n, mine, seat);
     kv8_f16x8 q[KC][2];
-    r.queries(a, w.s, q);
-    const char* mask = MASK ? a.mask + (int64_t)r.j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
+    Rows<D>::queries(a, w.s, seat, q);
+    const char* masks = MASK ? a.mask + (int64_t)w.s * a.m_nb3 : nullptr;
+    const int j = seat.j;
     int last = w.last;  // blocks that any row of the work-group sees
     if (a.mode == SIXI_MASK_BLOCK_CAUSAL)
         last = min(last, (w.n.cached + (min(r0 + 32 * NW, w.n.rows * a.G) - 1) / a.G + kBlk) / kBlk);
     if (w.first < last) {
-        const uint32_t k_off = h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
-        const uint32_t v_off = n * kBlk + h * 16;
         // The wave's share of the next step's codes, on their way.  At 256 dims K and V go through the same
         // registers, K in the first half of a step and V in the second.
         constexpr bool kOne = D == 256;
@@ -588,7 +597,10 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
             int step = both ? (which ? walk.v_nb : walk.k_nb) : 0;
             asm("" : "+s"(step));
             const char* p = which ? walk.v : walk.k;
-            const uint32_t off = which ? v_off : k_off;
+            int at = lane;
+            if (kOne) asm volatile("" : "+v"(at));  // (formed again: kept, they take registers that 256 dims lack)
+            const int n = at & 31, h = at >> 5;
+            const uint32_t off = which ? n * kBlk + h * 16 : h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
                 const int it = wave + i * NW;
@@ -639,10 +651,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                 walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
             }
             f16x8u add[NB][2];
-            if (any) {
-                if (MASK)
+            auto load_mask = [&]() {
+                int row = j;  // (a row's address is formed again: kept, it takes two registers)
+                asm volatile("" : "+v"(row));
+                const char* mask = masks + (int64_t)row * a.m_nb1;
 #pragma unroll
-                    for (int i = 0; i < NB; ++i) Rows<D>::mask_of(mask, min(b + i, last - 1), add[i]);
+                for (int i = 0; i < NB; ++i) Rows<D>::mask_of(mask, min(b + i, last - 1), add[i]);
+            };
+            if (any) {
+                if (MASK && !kOne) load_mask();
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -656,6 +673,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (kOne) {
+                if (MASK && any) load_mask();  // (behind the products: beside their operands there is no room)
                 convert(buf ^ 1, 0);
                 load(1);
                 load_exps();
@@ -710,10 +728,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
         }
     }
     r.l = sum_halves(r.l);
+    asm volatile("" : "+s"(mine));  // (the seat is looked up again: kept, it takes registers from the loop)
+    seat = seat_of(a, w.n, w.g, mine);
     if (w.pieces == 1)
-        r.finish(a, w.s);
+        r.finish(a, w.s, seat);
     else
-        r.leave(a.part + ((int64_t)w.id * NW + wave) * tile_floats(D));
+        r.leave(a.part + ((int64_t)w.id * NW + wave) * tile_floats(D), seat);
 }
 
 // Joins the pieces of 32 rows: D/32 work-groups of four waves, each with 4 of the accumulators' D/8 quads.  What a
