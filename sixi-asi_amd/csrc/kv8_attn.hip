@@ -369,6 +369,12 @@ __device__ __forceinline__ bool work_of(const Kv8AttnArgs& a, Work& w) {
 
 constexpr int kWaves = 4;
 
+// T tiles of 32 rows in the registers of every wave, the waves on cells of their own; joined through LDS at the end.
+//
+// Bound by memory where streams are many or long: one token of 32 streams behind 0.5k to 16k cells, 128 dims, 269 MB:
+// 47 us, 5.7 TB/s, and 61 with the launch, the cut and the merge.  Bound by latency where they are not: one token
+// behind 4095 cells, 256 dims: 10 us (lengths and cut 2, codes and queries, four waves' join) and the merge's 5.
+// Two tiles are a rule of kv8_attn_plan.
 template <int D, int T, bool MASK>
 __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_kernel(Kv8AttnArgs a) {
     constexpr int KC = D / 32;
@@ -538,8 +544,6 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
     }
 }
 
-// Four waves of 32 rows each over the same cells, NB blocks of 32 a step.  A wave without rows still converts
-// its share of the codes: three waves of rows and one without measured faster than a work-group of three.
 // N products whose left operands come from LDS: A reads first, then two more with every two products, so that a
 // read has the time of A - 2 products to arrive.
 template <int N, int A>
@@ -557,6 +561,16 @@ constexpr size_t rows_lds() {
     return (size_t)2 * 2 * NB * (D / 32) * 2 * 64 * 16;
 }
 
+// Four waves of 32 rows each over the same cells, NB blocks of 32 a step.  A wave without rows still converts
+// its share of the codes: three waves of rows and one without measured faster than a work-group of three.
+//
+// Bound by instructions, not by memory: a wave's 32 x 32 scores and their product with V are 16 MFMAs of 32 cycles
+// (128 dims) next to some 70 VALU instructions of softmax, 16 of them exponentials at a quarter of the rate, and a
+// quarter of the conversions.  2048 rows behind 4096 cells, 128 dims: 181 us, 714 TFLOP/s; the matrix cores are busy
+// for 28 % of the time and the VALU for 39 %, two waves of a SIMD overlap them in part, and the chunk's 384 work-groups
+// leave half of the CUs with one instead of two.  96 rows of 32 streams, up to 16k cells: 101 us (2.7 TB/s).
+// 256 dims leave registers for one tensor's codes on their way: 173 rows behind 11400 cells 81 us, 600 TFLOP/s;
+// trees of 12 tokens, 8 streams up to 9k cells, 57 us.
 template <int D, int NB, bool MASK>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnArgs a) {
     constexpr int NW = kWaves;

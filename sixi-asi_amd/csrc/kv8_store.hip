@@ -12,6 +12,10 @@
 // 4 x 4 in registers into 4 dims' cells), all without bank conflicts, so that every access to the cache is 16
 // bytes and a whole block leaves as one piece.  (With V's bytes scattered into LDS one by one a chunk of 2048
 // rows of 256 took 13 us instead of 8, and its read-back 13 instead of 5.)
+//
+// Measured: 2048 f16 rows of 4 heads of 256 dims 8.2 us (13 MB in and out, 1.5 TB/s: four work-groups a CU, one round
+// of loads, reductions and stores), read back 5.5 us; a token of 32 streams 6.4 us, read back 4.0: launch and two
+// dependent loads.
 #include "kv8_device.hpp"
 
 namespace sixi {

@@ -9,7 +9,8 @@
 // 8 consecutive elements per lane, D/8 lanes a head row: 16 or 32 bytes of loads and stores per lane.  The
 // partner of an element in the half layout sits n_rot/16 lanes away, in the same register; interleaved
 // pairs lie within a lane.  The norm's sum of squares is a sum over the row's lanes.  Every element is read
-// by the lane that writes it, so the output may be the input.  HBM-bound: rows in and out once.
+// by the lane that writes it, so the output may be the input.  HBM-bound: rows in and out once: 2048 f16 rows
+// of 28 heads of 128 dims 9.4 us (29 MB, 3.1 TB/s); a token 4 us, which is a launch, a length and its rows.
 #include <hip/hip_runtime.h>
 
 #include "rope_internal.hpp"
@@ -136,7 +137,7 @@ hipError_t launch_qk_rope(const RopeArgs& a, hipStream_t stream) {
     const int heads = a.t[0].heads + a.t[1].heads;
     if (a.n_rows == 0 || a.S == 0 || heads == 0) return hipSuccess;
     // few rows: a work-group for each group of heads that its lanes hold at once (their angles formed again
-    // cost less than waiting for one group after another: a token of 28 heads 7.8 -> 4.0 us)
+    // cost less than waiting for one group after another: a token of 28 heads 7.8 us and 4.0 so)
     const int per = kThreads / (a.D > 128 ? 32 : a.D > 64 ? 16 : 8), passes = (heads + per - 1) / per;
     const dim3 grid((unsigned)a.n_rows, (int64_t)a.n_rows * a.S <= 1024 ? (unsigned)passes : 1u, (unsigned)a.S);
     if (a.D > 128)
