@@ -141,6 +141,17 @@ struct Cut {
             c = (int)((float)c * fminf((float)total / (float)a.target, 1.5f)) / 2 * 2 + 2;
         }
     }
+    // The same for a call of one stream.
+    __device__ __forceinline__ void alone(const Kv8AttnArgs& a, Place& p) {
+        const Lens n = lens_of(a, 0);
+        const int t = (n.rows * a.G + 32 * a.waves - 1) / (32 * a.waves), blocks = blocks_of(n), all = t * a.Hkv;
+        // as many pieces as fit the places beside the other tiles and heads
+        const int most = enough(t, a) ? 1 : a.target / max(all, 1);
+        c = (max((blocks + most - 1) / most, a.least) + 1) / 2 * 2;
+        p.tiles = t;
+        p.pieces = max(1, (blocks + c - 1) / c);
+        total = all * p.pieces;
+    }
     // The stream that holds piece `id`.
     __device__ __forceinline__ Place find(const Kv8AttnArgs& a, int id) {
         const int lane = threadIdx.x & 63, sum = total;
@@ -349,11 +360,17 @@ struct Work {
     Lens n;
 };
 __device__ __forceinline__ bool work_of(const Kv8AttnArgs& a, Work& w) {
-    Cut cut;
-    cut.begin(a);
     w.id = blockIdx.x;
-    if (w.id >= cut.total) return false;
-    const Place p = cut.find(a, w.id);
+    Cut cut;
+    Place p{0, 1, 1, 0};
+    if (a.S == 1) {  // one stream needs no sums over streams (15.5 against XX us for a token behind 4095 cells)
+        cut.alone(a, p);
+        if (w.id >= cut.total) return false;
+    } else {
+        cut.begin(a);
+        if (w.id >= cut.total) return false;
+        p = cut.find(a, w.id);
+    }
     if (a.cut && w.id == p.at && threadIdx.x == 0) a.places[p.s] = p;  // for the merge
     w.s = p.s;
     w.pieces = p.pieces;
@@ -758,11 +775,10 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a) {
     __shared__ __align__(16) kv8_f32x4 sums[kWaves][4][64];
     __shared__ float tops[kWaves][32], totals[kWaves][32];
     const int s = blockIdx.z, g = blockIdx.y, quads = blockIdx.x % (D / 32), t32 = blockIdx.x / (D / 32);
+    const Place p = a.places[s];  // (asked for with the lengths: a stream without rows has left none, and reads none)
     const Lens len = lens_of(a, s);
     const int M = len.rows * a.G;
-    if (t32 * 32 >= M) return;
-    const Place p = a.places[s];
-    if (p.pieces == 1) return;
+    if (t32 * 32 >= M || p.pieces == 1) return;
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int quad = quads * 4 + wave, rr = t32 * 32 + n;
