@@ -223,6 +223,24 @@ def test_draft_verify_strides_and_misaligned_rows():
     assert [keep.tolist(), token.tolist()] == _want(c)
 
 
+def test_draft_verify_rows_past_32_bits():
+    """Rows of logits and of the drafter's distribution three GiB apart."""
+    c = _case(1, 3, 5000, True, 44)
+    step = 3 << 28                                        # in f32 elements
+    want = _run(c)
+    assert list(want) == _want(c)
+    wide = torch.empty(2 * step + 5000, device="cuda")
+    logits = wide.as_strided((1, 3, 5000), (wide.numel(), step, 1))
+    logits.copy_(c["logits"])
+    more = torch.empty(step + 5000, device="cuda")
+    probs = more.as_strided((1, 2, 5000), (more.numel(), step, 1))
+    probs.copy_(torch.from_numpy(c["probs"]))
+    keep, token = (torch.full((1,), -7, dtype=torch.int32, device="cuda") for _ in range(2))
+    sa.DraftVerify()(logits, torch.from_numpy(c["draft"]).cuda(), torch.from_numpy(c["u"]).cuda(), torch.from_numpy(c["u_next"]).cuda(),
+                     keep, token, draft_probs=probs, temperature=torch.from_numpy(c["heat"]).cuda())
+    assert (keep.tolist(), token.tolist()) == want
+
+
 def test_draft_verify_draws_as_the_target_would():
     """Over 20000 draws of a two-row block the first token is distributed as p (both the kept and the drawn)."""
     V, N = 8, 20000

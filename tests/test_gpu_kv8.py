@@ -260,6 +260,49 @@ def test_attention_of_33_to_96_rows(d, n_q, H, heads):
         _attend(2, n_q, H, heads, d, [800, 90], [n_q, n_q], 1024, mode=sa.MASK_EXPLICIT, mask=m, seed=5)
 
 
+@pytest.mark.parametrize("s", [64, 65, 130, 512])
+def test_attention_of_many_streams(s):
+    """Past 64 streams the cut goes over the lanes more than once."""
+    rng = np.random.default_rng(s)
+    cached = [int(x) for x in rng.integers(0, 250, s)]
+    rows = [int(x) for x in rng.integers(0, 3, s)]
+    _attend(s, 2, 6, 1, 128, cached, rows, 256)
+    cached[s // 2], rows[s // 2] = 3000, 2      # one long among short ones: its pieces are numbered between theirs
+    cached[-1], rows[-1] = 1200, 1
+    _attend(s, 2, 2, 1, 128, cached, rows, 3104, seed=1)
+
+
+@pytest.mark.parametrize("d,n_q", [(128, 2), (128, 40), (256, 40)])
+def test_offsets_past_32_bits(d, n_q):
+    """Blocks half a GiB apart: a stream's cells lie up to 5 GiB behind one another."""
+    rng = np.random.default_rng(d + n_q)
+    cells, step = 320, 1 << 29
+    k, v = random_cells(rng, 1, cells, 1, d), random_cells(rng, 1, cells, 1, d)
+    packed = [*k.pack_key(), *v.pack_value()]
+    room = [torch.empty((cells // BLOCK - 1) * step + 2 * BLOCK * d, dtype=torch.int8, device="cuda") for _ in range(2)]
+    codes = []
+    for t, r in zip((packed[0], packed[2]), room):
+        inner = [x for x in t.stride()[3:]]
+        far = r.as_strided(t.shape, (r.numel(), BLOCK * d, step, *inner))
+        far.copy_(t)
+        codes.append(far)
+    cache = sa.Kv8Cache(codes[0], packed[1].cuda(), codes[1], packed[3].cuda())
+    rk, rv = _rows(rng, 1, 40, 1, d, False), _rows(rng, 1, 40, 1, d, False)
+    first = cells - 41
+    sa.kv8_write(torch.from_numpy(rk).cuda(), torch.from_numpy(rv).cuda(), cache, kv_len=_i32([first]))
+    k.write(rk.astype(np.float64), [first], [40])
+    v.write(rv.astype(np.float64), [first], [40])
+    back = [torch.zeros((1, cells, 1, d), device="cuda") for _ in range(2)]
+    sa.kv8_read(cache, *back)
+    for got, want in zip(back, (k, v)):
+        assert np.array_equal(got.cpu().numpy(), want.values().astype(np.float32))
+    q = rng.standard_normal((1, n_q, 3, d)).astype(np.float16)
+    out = torch.zeros((1, n_q, 3, d), device="cuda")
+    sa.Kv8Attention()(torch.from_numpy(q).cuda(), cache, out, kv_len=_i32([cells - 1 - n_q]))
+    want, tol = attention(q.astype(np.float64), k.values(), v.values(), v.exps, [cells - 1 - n_q], [n_q], d ** -0.5, sa.MASK_BLOCK_CAUSAL)
+    assert (np.abs(out.double().cpu().numpy() - want) <= tol + 2.0 ** -22 * np.abs(want)).all()
+
+
 def test_attention_few_rows_of_a_long_block():
     """Rows for many tiles, few of them there: their cells are cut and joined."""
     _attend(2, 2000, 24, 4, 128, [1500, 2000], [40, 3], 4096)

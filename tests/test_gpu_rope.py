@@ -125,6 +125,19 @@ def test_rope_gradient_is_the_inverse_rotation():
         assert np.abs(got.cpu().double().numpy() - grad).max() <= 32 * 2.0 ** -24 * 2 * float(g.abs().max()) + 1e-9
 
 
+def test_rope_rows_past_32_bits():
+    """Rows three GiB apart, in place."""
+    d, step = 64, 3 << 28                                 # in f32 elements
+    wide = torch.empty(2 * step + 2 * d, device="cuda")
+    q = wide.as_strided((1, 3, 2, d), (wide.numel(), step, d, 1))
+    q.copy_(torch.randn((1, 3, 2, d), generator=torch.Generator().manual_seed(5)))
+    before = q.clone()
+    freqs, _ = sa.rope_frequencies(32, 1e4)
+    sa.qk_rope(q, None, freqs, kv_len=_i32([77]))
+    want, size = _reference(before.double().cpu().numpy(), freqs.cpu().numpy(), 77 + np.arange(3)[None], 0, 1.0, None)
+    _check(q, want, size, np.ones((1, 3), bool), "far rows")
+
+
 def test_rope_writes_rows_of_their_own_only():
     """Every second row of a buffer: the rows between stay."""
     q = torch.randn((1, 4, 3, 128), device="cuda")
