@@ -19,7 +19,7 @@
 // lane needs as its half of the next product's right operand.  So P never leaves its lane.
 //
 // Two kernels.  Up to 32 rows a group (decode), or 64 of 128 dims: the four waves of a work-group take blocks
-// in turn, straight from memory into registers, one block ahead; nothing is shared but two tiles' queries.
+// in turn, straight from memory into registers, one block ahead; nothing is shared but the queries.
 // More rows: NW waves take 32 rows each of the same cells; a step's codes are converted once, by all of them,
 // into f16 operands in LDS (two buffers, the next step's codes on their way in registers).
 //
@@ -228,32 +228,30 @@ struct Rows {
         l = 0.0f;
     }
 
-    // The rows' queries as the products' right operands.
-    __device__ __forceinline__ static void queries(const Kv8AttnArgs& a, int s, const Seat& seat, kv8_f16x8 (&q)[KC][2]) {
+    // The rows' queries, 32 dims of them, as a product's right operands.
+    __device__ __forceinline__ static void queries(const Kv8AttnArgs& a, int s, const Seat& seat, int c, kv8_f16x8 (&q)[2]) {
         const int h = (threadIdx.x & 63) >> 5;
         const char* p = a.q + (int64_t)seat.j * a.q_nb1 + (int64_t)seat.head * a.q_nb2 + (int64_t)s * a.q_nb3;
 #pragma unroll
-        for (int c = 0; c < KC; ++c)
+        for (int u = 0; u < 2; ++u) {
+            const int d = (2 * c + h) * 16 + 8 * u;
+            kv8_f16x8 x = {};
+            if (seat.live) {
+                if (a.q_f16) {
+                    x = *reinterpret_cast<const kv8_f16x8*>(p + d * 2);
+                } else {
+                    const kv8_f32x4 lo = *reinterpret_cast<const kv8_f32x4*>(p + d * 4);
+                    const kv8_f32x4 hi = *reinterpret_cast<const kv8_f32x4*>(p + d * 4 + 16);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int d = (2 * c + h) * 16 + 8 * u;
-                kv8_f16x8 x = {};
-                if (seat.live) {
-                    if (a.q_f16) {
-                        x = *reinterpret_cast<const kv8_f16x8*>(p + d * 2);
-                    } else {
-                        const kv8_f32x4 lo = *reinterpret_cast<const kv8_f32x4*>(p + d * 4);
-                        const kv8_f32x4 hi = *reinterpret_cast<const kv8_f32x4*>(p + d * 4 + 16);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[i] = (_Float16)lo[i];
-                            x[4 + i] = (_Float16)hi[i];
-                        }
+                    for (int i = 0; i < 4; ++i) {
+                        x[i] = (_Float16)lo[i];
+                        x[4 + i] = (_Float16)hi[i];
                     }
-                    x = x * (_Float16)a.q_sign;
                 }
-                q[c][u] = x;
+                x = x * (_Float16)a.q_sign;
             }
+            q[u] = x;
+        }
     }
 
     // The mask's values for the lane's 16 cells of a block (all of a block's are there, whatever the row sees).
@@ -363,7 +361,7 @@ __device__ __forceinline__ bool work_of(const Kv8AttnArgs& a, Work& w) {
     w.id = blockIdx.x;
     Cut cut;
     Place p{0, 1, 1, 0};
-    if (a.S == 1) {  // one stream needs no sums over streams (a token behind 4095 cells: 15.0 us, and 15.4 with them)
+    if (a.S == 1) {  // one stream needs no sums over streams (0.4 us of a token behind 4095 cells)
         cut.alone(a, p);
         if (w.id >= cut.total) return false;
     } else {
@@ -387,13 +385,17 @@ __device__ __forceinline__ bool work_of(const Kv8AttnArgs& a, Work& w) {
 constexpr int kWaves = 4;
 
 // T tiles of 32 rows in the registers of every wave, the waves on cells of their own; joined through LDS at the end.
+// The queries are read from LDS in every step and K is converted piece by piece beside its products: with the
+// accumulators that leaves room for two work-groups on a CU at 256 dims too, i.e. twice the codes on their way
+// (32 streams behind 0.5k to 8k cells, 256 dims: 66 us, and 72 with the queries in registers and one).
 //
 // Bound by memory where streams are many or long: one token of 32 streams behind 0.5k to 16k cells, 128 dims, 269 MB:
 // 47 us, 5.7 TB/s, and 61 with the launch, the cut and the merge.  Bound by latency where they are not: one token
-// behind 4095 cells, 256 dims: 10 us (lengths and cut 2, codes and queries, four waves' join) and the merge's 5.
+// behind 4095 cells, 256 dims: 14.2 us with the merge, of it lengths and cut 1.3, codes and queries 2.8, the step 2,
+// the four waves' join 2.
 // Two tiles are a rule of kv8_attn_plan.
 template <int D, int T, bool MASK>
-__global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_kernel(Kv8AttnArgs a) {
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_few_kernel(Kv8AttnArgs a) {
     constexpr int KC = D / 32;
     extern __shared__ __align__(16) float lds[];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
@@ -432,24 +434,19 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
         r[t].begin(a, w.n, r0 + t * 32, seat[t]);
         mask[t] = MASK ? a.mask + (int64_t)seat[t].j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
     }
-    kv8_f16x8 q[KC][2];
-    // several tiles' queries stay in LDS, for all waves: [tile][piece][first, second eight][lane]
+    // the queries stay in LDS, for all waves, each of which fetches a share: [tile][piece][first, second eight][lane]
     typedef kv8_f16x8 Queries[KC][2][64];
     Queries* qs = reinterpret_cast<Queries*>(lds);
-    if constexpr (T == 1) {
-        Rows<D>::queries(a, w.s, seat[0], q);
-    } else {
 #pragma unroll
-        for (int t = 0; t < T; ++t)
-            if (wave == t) {
-                Rows<D>::queries(a, w.s, seat[t], q);
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-                for (int c = 0; c < KC; ++c)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) qs[t][c][u][lane] = q[c][u];
-            }
-        __syncthreads();
-    }
+        for (int c = 0; c < KC; c += kWaves) {
+            kv8_f16x8 q[2];
+            Rows<D>::queries(a, w.s, seat[t], c + wave, q);
+            qs[t][c + wave][0][lane] = q[0];
+            qs[t][c + wave][1][lane] = q[1];
+        }
+    __syncthreads();
     if (b < last) {
         f16x8u add[T][2], next[T][2];
         if (MASK)
@@ -459,15 +456,20 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
         for (; b < last; b += kWaves) {
             f32x16 sc[T] = {};
             int at = lane;  // (read from LDS in every step: out of the loop they would fill the registers)
-            if (T > 1) asm volatile("" : "+v"(at));
-            kv8_f16x8 x[KC][2];
-#pragma unroll
-            for (int c = 0; c < KC; ++c) codes_f16x16(kc[c], x[c][0], x[c][1]);
+            asm volatile("" : "+v"(at));
             const int ek0 = clamp_exp(ek), ev0 = clamp_exp(ev);
-#pragma unroll
-            for (int c = 0; c < KC; ++c) kc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.k + k_off + c * (kBlk * 32));
             ek = *walk.ke;
             ev = *walk.ve;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                kv8_f16x8 x[2];
+                codes_f16x16(kc[c], x[0], x[1]);
+                kc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.k + k_off + c * (kBlk * 32));
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int t = 0; t < T; ++t) sc[t] = mfma(x[u], qs[t][c][u][at], sc[t]);
+            }
             if (MASK)
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
@@ -477,12 +479,6 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
                 }
             const char* vn = walk.v;
             walk.go(a.pages, a.k, a.v, w.s, w.g, kWaves);
-#pragma unroll
-            for (int c = 0; c < KC; ++c)
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int t = 0; t < T; ++t) sc[t] = mfma(x[c][u], T == 1 ? q[c][u] : qs[t][c][u][at], sc[t]);
             const float ks = a.scale_log2 * exp2_int(ek0), es = (float)ev0;
             float top[T];
 #pragma unroll
@@ -521,40 +517,58 @@ __global__ __launch_bounds__(kWaves * 64, D == 128 ? 2 : 1) void kv8_attn_few_ke
             }
         }
     }
+    // the waves' results into LDS, half of the accumulators at a time, and a quarter of them out of it for each wave
+    constexpr int kHalf = KC / 2, kPlace = kHalf * 4 * 64 * 4 + 64;
 #pragma unroll
     for (int t = 0; t < T; ++t) {
         r[t].l = sum_halves(r[t].l);
-        // the waves' results into LDS, and a quarter of the accumulators out of it for each wave
-        if (T > 1) __syncthreads();
-        r[t].leave(lds + wave * tile_floats(D), seat[t]);
-        __syncthreads();
-        if (!seat[t].live) continue;
         float m = kLowest, l = 0.0f, f[kWaves];
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-            f[k] = lds[k * tile_floats(D) + 32 * D + n];
-            m = fmaxf(m, f[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-            f[k] = __builtin_amdgcn_exp2f(f[k] - m);
-            l = fmaf(lds[k * tile_floats(D) + 32 * D + 32 + n], f[k], l);
-        }
-        const float inv = w.pieces > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
         char* row = a.out + (int64_t)seat[t].head * a.o_nb1 + (int64_t)seat[t].j * a.o_nb2 + (int64_t)w.s * a.o_nb3;
         float* part = a.part + ((int64_t)w.id * T + t) * tile_floats(D);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const int quad = wave * (D / 32) + i;
-            kv8_f32x4 x = {};
+        for (int half = 0; half < 2; ++half) {
+            __syncthreads();  // (what was there has been read)
+            if (seat[t].live) {
 #pragma unroll
-            for (int k = 0; k < kWaves; ++k) x += *reinterpret_cast<const kv8_f32x4*>(lds + k * tile_floats(D) + (quad * 64 + lane) * 4) * f[k];
-            if (w.pieces > 1)
-                *reinterpret_cast<kv8_f32x4*>(part + (quad * 64 + lane) * 4) = x;
-            else
-                store4(a, row, quad / 4 * 32 + quad % 4 * 8 + 4 * h, x * inv);
+                for (int c = 0; c < kHalf; ++c)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const f32x16& o = r[t].o[half * kHalf + c];
+                        *reinterpret_cast<kv8_f32x4*>(lds + wave * kPlace + ((c * 4 + i / 4) * 64 + lane) * 4) = kv8_f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+                    }
+                if (half == 0 && h == 0) {
+                    lds[wave * kPlace + kPlace - 64 + n] = r[t].m;
+                    lds[wave * kPlace + kPlace - 32 + n] = r[t].l;
+                }
+            }
+            __syncthreads();
+            if (!seat[t].live) continue;
+            if (half == 0) {
+#pragma unroll
+                for (int k = 0; k < kWaves; ++k) {
+                    f[k] = lds[k * kPlace + kPlace - 64 + n];
+                    m = fmaxf(m, f[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < kWaves; ++k) {
+                    f[k] = __builtin_amdgcn_exp2f(f[k] - m);
+                    l = fmaf(lds[k * kPlace + kPlace - 32 + n], f[k], l);
+                }
+            }
+            const float inv = w.pieces > 1 ? 1.0f : l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) {
+                const int at = wave * kHalf + i, quad = half * kHalf * 4 + at;
+                kv8_f32x4 x = {};
+#pragma unroll
+                for (int k = 0; k < kWaves; ++k) x += *reinterpret_cast<const kv8_f32x4*>(lds + k * kPlace + (at * 64 + lane) * 4) * f[k];
+                if (w.pieces > 1)
+                    *reinterpret_cast<kv8_f32x4*>(part + (quad * 64 + lane) * 4) = x;
+                else
+                    store4(a, row, quad / 4 * 32 + quad % 4 * 8 + 4 * h, x * inv);
+            }
         }
-        if (w.pieces > 1 && wave == 0 && h == 0) {
+        if (seat[t].live && w.pieces > 1 && wave == 0 && h == 0) {
             part[32 * D + n] = m;
             part[32 * D + 32 + n] = l;
         }
@@ -608,7 +622,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
     Rows<D> one[1], &r = one[0];
     r.begin(a, w.n, mine, seat);
     kv8_f16x8 q[KC][2];
-    Rows<D>::queries(a, w.s, seat, q);
+#pragma unroll
+    for (int c = 0; c < KC; ++c) Rows<D>::queries(a, w.s, seat, c, q[c]);
     const char* masks = MASK ? a.mask + (int64_t)w.s * a.m_nb3 : nullptr;
     const int j = seat.j;
     int last = w.last;  // blocks that any row of the work-group sees
@@ -859,7 +874,8 @@ __global__ __launch_bounds__(256) void kv8_merge_kernel(Kv8AttnArgs a) {
 
 template <int D, int T, bool MASK>
 void launch_few(const Kv8AttnArgs& a, hipStream_t stream) {
-    const size_t lds = (size_t)kWaves * tile_floats(D) * sizeof(float);
+    constexpr size_t lds = (size_t)kWaves * (16 * D + 64) * sizeof(float);
+    static_assert(lds >= (size_t)T * (D / 32) * 2 * 64 * 16, "the queries lie where the results are joined");
     hipLaunchKernelGGL((kv8_attn_few_kernel<D, T, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
 }
 template <int D, bool MASK>
@@ -895,7 +911,7 @@ size_t kv8_attn_plan(Kv8AttnArgs& a) {
     // do not fit beside them (32 streams of 60 rows: 175 against 118 us).
     const bool two = t32 == 2 && a.D == 128 && a.mode != SIXI_MASK_EXPLICIT;
     a.waves = t32 == 1 ? 1 : two ? 2 : kWaves;
-    a.target = 2 * device_cu_count();
+    a.target = 2 * device_cu_count();  // (two work-groups on a CU)
     a.least = 4;
     const int64_t tiles = (t32 + a.waves - 1) / a.waves * a.Hkv * a.S;
     const int64_t blocks = (a.n_kv + kBlk - 1) / kBlk;
