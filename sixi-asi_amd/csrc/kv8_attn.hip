@@ -587,11 +587,6 @@ __device__ __forceinline__ void feed() {
     }
 }
 
-template <int D, int NB>
-constexpr size_t rows_lds() {
-    return (size_t)2 * 2 * NB * (D / 32) * 2 * 64 * 16;
-}
-
 // Four waves of 32 rows each over the same cells, NB blocks of 32 a step.  A wave without rows still converts
 // its share of the codes: three waves of rows and one without measured faster than a work-group of three.
 //
@@ -600,13 +595,13 @@ constexpr size_t rows_lds() {
 // quarter of the conversions.  2048 rows behind 4096 cells, 128 dims: 181 us, 714 TFLOP/s; the matrix cores are busy
 // for 28 % of the time and the VALU for 39 %, two waves of a SIMD overlap them in part, and the chunk's 384 work-groups
 // leave half of the CUs with one instead of two.  96 rows of 32 streams, up to 16k cells: 101 us (2.7 TB/s).
-// 256 dims leave registers for one tensor's codes on their way: 173 rows behind 11400 cells 81 us, 600 TFLOP/s;
-// trees of 12 tokens, 8 streams up to 9k cells, 57 us.
-template <int D, int NB, bool MASK>
-__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnArgs a) {
-    constexpr int NW = kWaves;
+constexpr int kStep128 = 2;  // blocks of a step
+constexpr size_t kLds128 = (size_t)2 * 2 * kStep128 * (128 / 32) * 2 * 64 * 16;
+template <bool MASK>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows128_kernel(Kv8AttnArgs a) {
+    constexpr int D = 128, NB = kStep128, NW = kWaves;
     constexpr int KC = D / 32, ITEMS = NB * KC, MINE = ITEMS / NW;
-    constexpr int kAhead = D == 128 ? 6 : 3;  // LDS reads ahead of their products
+    constexpr int kAhead = 6;  // LDS reads ahead of their products
     static_assert(ITEMS % NW == 0, "every wave converts the same share");
     extern __shared__ __align__(16) float lds[];
     // [buffer][K, V][block, piece][first, second eight][lane] 8 f16
@@ -624,16 +619,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
     kv8_f16x8 q[KC][2];
 #pragma unroll
     for (int c = 0; c < KC; ++c) Rows<D>::queries(a, w.s, seat, c, q[c]);
-    const char* masks = MASK ? a.mask + (int64_t)w.s * a.m_nb3 : nullptr;
-    const int j = seat.j;
+    const char* mask = MASK ? a.mask + (int64_t)seat.j * a.m_nb1 + (int64_t)w.s * a.m_nb3 : nullptr;
     int last = w.last;  // blocks that any row of the work-group sees
     if (a.mode == SIXI_MASK_BLOCK_CAUSAL)
         last = min(last, (w.n.cached + (min(r0 + 32 * NW, w.n.rows * a.G) - 1) / a.G + kBlk) / kBlk);
     if (w.first < last) {
-        // The wave's share of the next step's codes, on their way.  At 256 dims K and V go through the same
-        // registers, K in the first half of a step and V in the second.
-        constexpr bool kOne = D == 256;
-        kv8_u32x4 codes[kOne ? 1 : 2][MINE];
+        kv8_u32x4 codes[2][MINE];  // the wave's share of the next step's, on their way
         int ek[NB], ev[NB];
         BlockWalk walk;
         // the walk's step; a second block that is none is the first once more (its cells are hidden).  The
@@ -643,14 +634,12 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
             int step = both ? (which ? walk.v_nb : walk.k_nb) : 0;
             asm("" : "+s"(step));
             const char* p = which ? walk.v : walk.k;
-            int at = lane;
-            if (kOne) asm volatile("" : "+v"(at));  // (formed again: kept, they take registers that 256 dims lack)
-            const int n = at & 31, h = at >> 5;
+            const int n = lane & 31, h = lane >> 5;
             const uint32_t off = which ? n * kBlk + h * 16 : h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
                 const int it = wave + i * NW;
-                codes[kOne ? 0 : which][i] = *reinterpret_cast<const kv8_u32x4*>(p + ((NB > 1 && it >= KC ? step : 0) + it % KC * (kBlk * 32)) + off);
+                codes[which][i] = *reinterpret_cast<const kv8_u32x4*>(p + ((it >= KC ? step : 0) + it % KC * (kBlk * 32)) + off);
             }
         };
         auto load_exps = [&]() {
@@ -670,7 +659,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
                 kv8_f16x8 x, y;
-                codes_f16x16(codes[kOne ? 0 : which][i], x, y);
+                codes_f16x16(codes[which][i], x, y);
                 tile[buf][which][wave + i * NW][0][lane] = x;
                 tile[buf][which][wave + i * NW][1][lane] = y;
             }
@@ -690,22 +679,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
             const bool any = b * kBlk < r.reach;
             f32x16 sc[NB] = {};
             // (behind the last step: its blocks once more, and not used)
-            if (!kOne) {
-                load(0);
-                load(1);
-                load_exps();
-                walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
-            }
+            load(0);
+            load(1);
+            load_exps();
+            walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
             f16x8u add[NB][2];
-            auto load_mask = [&]() {
-                int row = j;  // (a row's address is formed again: kept, it takes two registers)
-                asm volatile("" : "+v"(row));
-                const char* mask = masks + (int64_t)row * a.m_nb1;
-#pragma unroll
-                for (int i = 0; i < NB; ++i) Rows<D>::mask_of(mask, min(b + i, last - 1), add[i]);
-            };
             if (any) {
-                if (MASK && !kOne) load_mask();
+                if (MASK)
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) Rows<D>::mask_of(mask, min(b + i, last - 1), add[i]);
                 __builtin_amdgcn_sched_barrier(0);
                 __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -717,13 +699,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                 feed<2 * NB * KC, kAhead>();
                 __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
-            }
-            if (kOne) {
-                if (MASK && any) load_mask();  // (behind the products: beside their operands there is no room)
-                convert(buf ^ 1, 0);
-                load(1);
-                load_exps();
-                walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
             }
             if (any) {
                 kv8_f16x8 p[NB][2];
@@ -748,10 +723,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
                 __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (!kOne) convert(buf ^ 1, 0);
+            convert(buf ^ 1, 0);
             convert(buf ^ 1, 1);
             scales();
-            if (kOne) load(0);
             __syncthreads();
         };
         walk.begin(a.pages, a.k, a.v, w.s, w.g, w.first, last);
@@ -762,7 +736,6 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
         convert(0, 1);
         scales();
         walk.go(a.pages, a.k, a.v, w.s, w.g, NB);
-        if (kOne) load(0);
         __syncthreads();
         // steps in pairs, one for each buffer.  (A loop of its own for the steps whose cells every row sees took
         // 50 more registers, and with them the reads ahead: 203 against 182 us for the prompt chunk.)
@@ -780,6 +753,174 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows_kernel(Kv8AttnAr
         r.finish(a, w.s, seat);
     else
         r.leave(a.part + ((int64_t)w.id * NW + wave) * tile_floats(D), seat);
+}
+
+// The same at 256 dims, where accumulators and queries leave few registers: most of the queries in LDS, K and V one
+// buffer each, a block a step with two barriers: V becomes f16 beside the scores' products and the next K beside the
+// output's, so that both have their codes on the way for a whole step and nothing is left in scratch memory.
+//
+// Bound as at 128 dims, with a barrier for every 16 MFMAs.  Trees of 12 tokens, 8 streams of 2k to 9k cells: 51 us, and
+// 55 with the queries in registers, two buffers and one tensor's codes on their way (2 streams up to 50k cells 69 and
+// 79); 16 tokens of 16 streams up to 16k cells 99 and 102; 1024 rows behind 2048 cells 119 and 115; 173 rows
+// behind 11400 cells 81 us, 600 TFLOP/s, and 79.  Where rows are cut their f32 partial results cost as much again as
+// the codes: the merge is 12 us of the last.
+constexpr int kKept256 = 2;  // pieces of the queries in registers
+struct Lds256 {
+    kv8_f16x8 k[8][2][64], v[8][2][64];   // [piece][first, second eight][lane]
+    kv8_f16x8 q[kWaves][8 - kKept256][2][64];   // what a wave's registers do not keep of its queries
+};
+
+template <bool MASK>
+__global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows256_kernel(Kv8AttnArgs a) {
+    constexpr int D = 256, KC = D / 32, MINE = KC / kWaves, kKept = kKept256;
+    extern __shared__ __align__(16) float lds[];
+    Lds256& x = *reinterpret_cast<Lds256*>(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Work w;
+    if (!work_of(a, w)) return;
+    const int r0 = w.tile * (32 * kWaves);
+    int mine = r0 + wave * 32;
+    Seat seat = seat_of(a, w.n, w.g, mine);
+    Rows<D> one[1], &r = one[0];
+    r.begin(a, w.n, mine, seat);
+    kv8_f16x8 q[kKept][2];
+#pragma unroll
+    for (int c = 0; c < kKept; ++c) Rows<D>::queries(a, w.s, seat, c, q[c]);
+#pragma unroll
+    for (int c = kKept; c < KC; ++c) {
+        kv8_f16x8 y[2];
+        Rows<D>::queries(a, w.s, seat, c, y);
+        x.q[wave][c - kKept][0][lane] = y[0];
+        x.q[wave][c - kKept][1][lane] = y[1];
+    }
+    const char* masks = MASK ? a.mask + (int64_t)w.s * a.m_nb3 : nullptr;
+    const int j = seat.j;
+    int last = w.last;  // blocks that any row of the work-group sees
+    if (a.mode == SIXI_MASK_BLOCK_CAUSAL)
+        last = min(last, (w.n.cached + (min(r0 + 32 * kWaves, w.n.rows * a.G) - 1) / a.G + kBlk) / kBlk);
+    if (w.first < last) {
+        kv8_u32x4 kc[MINE], vc[MINE];
+        int ek, ev, e0;
+        float ks, es;
+        BlockWalk walk;
+        // (offsets are formed again at each use: kept, they take registers)
+        auto load_k = [&]() {
+            int at = lane;
+            asm volatile("" : "+v"(at));
+            const int n = at & 31, h = at >> 5;
+            const uint32_t off = h * (kBlk * 16) + (16 * (n / 4 % 2) + 4 * (n / 8) + n % 4) * 16;
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) kc[i] = *reinterpret_cast<const kv8_u32x4*>(walk.k + (wave + i * kWaves) * (kBlk * 32) + off);
+            ek = *walk.ke;
+            ev = *walk.ve;
+        };
+        auto load_v = [&]() {
+            int at = lane;
+            asm volatile("" : "+v"(at));
+            const uint32_t off = (at & 31) * kBlk + (at >> 5) * 16;
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) vc[i] = *reinterpret_cast<const kv8_u32x4*>(walk.v + (wave + i * kWaves) * (kBlk * 32) + off);
+        };
+        auto convert = [&](const kv8_u32x4 (&codes)[MINE], kv8_f16x8 (&to)[8][2][64]) {
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+                kv8_f16x8 lo, hi;
+                codes_f16x16(codes[i], lo, hi);
+                to[wave + i * kWaves][0][lane] = lo;
+                to[wave + i * kWaves][1][lane] = hi;
+            }
+        };
+        auto scales = [&]() {
+            ks = a.scale_log2 * exp2_int(clamp_exp(ek));
+            e0 = clamp_exp(ev);
+            es = (float)e0;
+        };
+        // (a scalar, so that branches on it are: waits for loads would count those of a path that no wave takes)
+        const int reach = __builtin_amdgcn_readfirstlane(r.reach);
+        walk.begin(a.pages, a.k, a.v, w.s, w.g, w.first, last);
+        load_k();
+        load_v();
+        convert(kc, x.k);
+        scales();
+        walk.go(a.pages, a.k, a.v, w.s, w.g, 1);
+        load_k();
+        __syncthreads();
+#pragma unroll 1
+        for (int b = w.first; b < last; ++b) {
+            const bool any = b * kBlk < reach;
+            f16x8u add[2];
+            kv8_f16x8 p[2];
+            f32x16 sc[1] = {};
+            if (any) {
+                if (MASK) {
+                    int row = j;
+                    asm volatile("" : "+v"(row));
+                    Rows<D>::mask_of(masks + (int64_t)row * a.m_nb1, b, add);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int c = 0; c < KC; ++c)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                        sc[0] = mfma(x.k[c][u][lane], c < kKept ? q[c < kKept ? c : 0][u] : x.q[wave][c < kKept ? 0 : c - kKept][u][lane], sc[0]);
+                convert(vc, x.v);
+                __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+                for (int i = 0; i < 2 * kKept - 3; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+                }
+#pragma unroll
+                for (int i = 2 * kKept - 3; i < 2 * KC; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                convert(vc, x.v);
+            }
+            load_v();  // (in one place: where two paths load, the registers are copied, which waits for them)
+            if (any) {
+                r.template hide<MASK>(sc[0], b, ks, es, add);
+                const float top[1] = {r.template top_of<MASK>(sc[0], ks, es)};
+                raise(one, top);
+                r.template weights<MASK>(sc[0], ks, es, e0, p);
+            }
+            scales();
+            walk.go(a.pages, a.k, a.v, w.s, w.g, 1);
+            __syncthreads();
+            if (any) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int c = 0; c < KC; ++c) r.o[c] = mfma(x.v[c][u][lane], p[u], r.o[c]);
+                convert(kc, x.k);
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+                for (int i = 0; i < 2 * KC; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            } else {
+                convert(kc, x.k);
+            }
+            load_k();
+            __syncthreads();
+        }
+    }
+    r.l = sum_halves(r.l);
+    asm volatile("" : "+s"(mine));  // (the seat is looked up again: kept, it takes registers from the loop)
+    seat = seat_of(a, w.n, w.g, mine);
+    if (w.pieces == 1)
+        r.finish(a, w.s, seat);
+    else
+        r.leave(a.part + ((int64_t)w.id * kWaves + wave) * tile_floats(D), seat);
 }
 
 // Joins the pieces of 32 rows: D/32 work-groups of four waves, each with 4 of the accumulators' D/8 quads.  What a
@@ -883,9 +1024,10 @@ void launch_pieces(const Kv8AttnArgs& a, hipStream_t stream) {
     if (a.waves == 1) return launch_few<D, 1, MASK>(a, stream);
     if constexpr (D == 128 && !MASK)
         if (a.waves == 2) return launch_few<D, 2, MASK>(a, stream);
-    constexpr int NB = D == 128 ? 2 : 1;
-    constexpr size_t lds = rows_lds<D, NB>();
-    hipLaunchKernelGGL((kv8_attn_rows_kernel<D, NB, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
+    if constexpr (D == 128)
+        hipLaunchKernelGGL(kv8_attn_rows128_kernel<MASK>, dim3((unsigned)a.grid), dim3(kWaves * 64), kLds128, stream, a);
+    else
+        hipLaunchKernelGGL(kv8_attn_rows256_kernel<MASK>, dim3((unsigned)a.grid), dim3(kWaves * 64), sizeof(Lds256), stream, a);
 }
 
 template <int D>
