@@ -592,9 +592,9 @@ __device__ __forceinline__ void feed() {
 //
 // Bound by instructions, not by memory: a wave's 32 x 32 scores and their product with V are 16 MFMAs of 32 cycles
 // (128 dims) next to some 70 VALU instructions of softmax, 16 of them exponentials at a quarter of the rate, and a
-// quarter of the conversions.  2048 rows behind 4096 cells, 128 dims: 181 us, 714 TFLOP/s; the matrix cores are busy
+// quarter of the conversions.  2048 rows behind 4096 cells, 128 dims: 178 us, 725 TFLOP/s; the matrix cores are busy
 // for 28 % of the time and the VALU for 39 %, two waves of a SIMD overlap them in part, and the chunk's 384 work-groups
-// leave half of the CUs with one instead of two.  96 rows of 32 streams, up to 16k cells: 101 us (2.7 TB/s).
+// leave half of the CUs with one instead of two.  96 rows of 32 streams, up to 16k cells: 99 us (2.8 TB/s).
 constexpr int kStep128 = 2;  // blocks of a step
 constexpr size_t kLds128 = (size_t)2 * 2 * kStep128 * (128 / 32) * 2 * 64 * 16;
 template <bool MASK>
@@ -759,11 +759,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_rows128_kernel(Kv8Att
 // buffer each, a block a step with two barriers: V becomes f16 beside the scores' products and the next K beside the
 // output's, so that both have their codes on the way for a whole step and nothing is left in scratch memory.
 //
-// Bound as at 128 dims, with a barrier for every 16 MFMAs.  Trees of 12 tokens, 8 streams of 2k to 9k cells: 51 us, and
+// Bound as at 128 dims, with a barrier for every 16 MFMAs.  Trees of 12 tokens, 8 streams of 2k to 9k cells: 50 us, and
 // 55 with the queries in registers, two buffers and one tensor's codes on their way (2 streams up to 50k cells 69 and
 // 79); 16 tokens of 16 streams up to 16k cells 99 and 102; 1024 rows behind 2048 cells 119 and 115; 173 rows
-// behind 11400 cells 81 us, 600 TFLOP/s, and 79.  Where rows are cut their f32 partial results cost as much again as
-// the codes: the merge is 12 us of the last.
+// behind 11400 cells 79 to 80 us, 610 TFLOP/s, and 79.  Where rows are cut their f32 partial results cost as much again as
+// the codes: the merge is 13 us of the last.
 constexpr int kKept256 = 2;  // pieces of the queries in registers
 struct Lds256 {
     kv8_f16x8 k[8][2][64], v[8][2][64];   // [piece][first, second eight][lane]
