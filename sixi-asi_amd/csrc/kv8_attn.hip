@@ -522,6 +522,9 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_few_kernel(Kv8AttnArg
 #pragma unroll
     for (int t = 0; t < T; ++t) {
         r[t].l = sum_halves(r[t].l);
+        int again = r0 + t * 32;
+        asm volatile("" : "+s"(again));  // (the seat is looked up again: kept, it takes registers from the loop)
+        seat[t] = seat_of(a, w.n, w.g, again);
         float m = kLowest, l = 0.0f, f[kWaves];
         char* row = a.out + (int64_t)seat[t].head * a.o_nb1 + (int64_t)seat[t].j * a.o_nb2 + (int64_t)w.s * a.o_nb3;
         float* part = a.part + ((int64_t)w.id * T + t) * tile_floats(D);

@@ -2,12 +2,14 @@
 status, before they touch a device; the frequency tables; what the Python binding refuses."""
 import ctypes
 import math
+import re
 
 import numpy as np
 import pytest
 import torch
 
 import sixi_attn as sa
+from test_asm_hazards import _asm_of, kernels_with_scratch
 
 FAKE = 0x7F0000000000  # aligned addresses far apart; validation never reads through them
 
@@ -527,3 +529,13 @@ def test_binding_refuses_host_tensors_and_wrong_types():
         sa.Kv8Cache(i8[0].transpose(3, 4).contiguous().transpose(3, 4), i8[1], i8[2], i8[3])
     with pytest.raises(ValueError, match="multiple of 32"):
         sa.Kv8Cache.empty(1, 100, 2, 128, device="cpu")
+
+
+# ---- the kernels as built ----
+
+@pytest.mark.parametrize("src", ["kv8_store.hip", "kv8_attn.hip", "rope.hip", "draft_verify.hip"])
+def test_kernels_use_no_scratch_and_no_packed_f32(src, tmp_path_factory):
+    asm = _asm_of(src, tmp_path_factory)
+    assert asm.count(".private_segment_fixed_size:") > 0
+    assert not kernels_with_scratch(asm)
+    assert not re.search(r"v_pk_(add|mul|fma)_f32", asm)
