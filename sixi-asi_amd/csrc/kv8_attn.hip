@@ -384,17 +384,24 @@ __device__ __forceinline__ bool work_of(const Kv8AttnArgs& a, Work& w) {
 
 constexpr int kWaves = 4;
 
+// 16 bytes of codes; ONCE: not to be kept in the caches.
+template <bool ONCE>
+__device__ __forceinline__ kv8_u32x4 codes_at(const char* p) {
+    const kv8_u32x4* x = reinterpret_cast<const kv8_u32x4*>(p);
+    return ONCE ? __builtin_nontemporal_load(x) : *x;
+}
+
 // T tiles of 32 rows in the registers of every wave, the waves on cells of their own; joined through LDS at the end.
 // The queries are read from LDS in every step and K is converted piece by piece beside its products: with the
 // accumulators that leaves room for two work-groups on a CU at 256 dims too, i.e. twice the codes on their way
-// (32 streams behind 0.5k to 8k cells, 256 dims: 66 us, and 72 with the queries in registers and one).
+// (32 streams behind 0.5k to 8k cells, 256 dims: 66 us, and 72 with the queries in registers and one; now 59).
 //
 // Bound by memory where streams are many or long: one token of 32 streams behind 0.5k to 16k cells, 128 dims, 269 MB:
-// 47 us, 5.7 TB/s, and 61 with the launch, the cut and the merge.  Bound by latency where they are not: one token
+// 53 us with the cut, the merge and its launch, 5.0 TB/s.  Bound by latency where they are not: one token
 // behind 4095 cells, 256 dims: 14.2 us with the merge, of it lengths and cut 1.3, codes and queries 2.8, the step 2,
 // the four waves' join 2.
-// Two tiles are a rule of kv8_attn_plan.
-template <int D, int T, bool MASK>
+// Two tiles, and loads that leave nothing in the caches (ONCE), are rules of kv8_attn_plan.
+template <int D, int T, bool MASK, bool ONCE>
 __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_few_kernel(Kv8AttnArgs a) {
     constexpr int KC = D / 32;
     extern __shared__ __align__(16) float lds[];
@@ -419,11 +426,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_few_kernel(Kv8AttnArg
     if (b < last) {
         walk.begin(a.pages, a.k, a.v, w.s, w.g, b, last);
 #pragma unroll
-        for (int c = 0; c < KC; ++c) kc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.k + k_off + c * (kBlk * 32));
+        for (int c = 0; c < KC; ++c) kc[c] = codes_at<ONCE>(walk.k + k_off + c * (kBlk * 32));
         ek = *walk.ke;
         ev = *walk.ve;
 #pragma unroll
-        for (int c = 0; c < KC; ++c) vc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.v + v_off + c * (kBlk * 32));
+        for (int c = 0; c < KC; ++c) vc[c] = codes_at<ONCE>(walk.v + v_off + c * (kBlk * 32));
     }
     Rows<D> r[T];
     Seat seat[T];
@@ -464,7 +471,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_few_kernel(Kv8AttnArg
             for (int c = 0; c < KC; ++c) {
                 kv8_f16x8 x[2];
                 codes_f16x16(kc[c], x[0], x[1]);
-                kc[c] = *reinterpret_cast<const kv8_u32x4*>(walk.k + k_off + c * (kBlk * 32));
+                kc[c] = codes_at<ONCE>(walk.k + k_off + c * (kBlk * 32));
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -494,7 +501,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_few_kernel(Kv8AttnArg
                 for (int c = 0; c < KC; ++c) {
                     kv8_f16x8 y[2];
                     codes_f16x16(vc[c], y[0], y[1]);
-                    vc[c] = *reinterpret_cast<const kv8_u32x4*>(vn + v_off + c * (kBlk * 32));
+                    vc[c] = codes_at<ONCE>(vn + v_off + c * (kBlk * 32));
                     r[0].o[c] = mfma(y[0], p[0], r[0].o[c]);
                     r[0].o[c] = mfma(y[1], p[1], r[0].o[c]);
                 }
@@ -503,7 +510,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void kv8_attn_few_kernel(Kv8AttnArg
 #pragma unroll
                 for (int c = 0; c < KC; ++c) {
                     codes_f16x16(vc[c], y[c][0], y[c][1]);
-                    vc[c] = *reinterpret_cast<const kv8_u32x4*>(vn + v_off + c * (kBlk * 32));
+                    vc[c] = codes_at<ONCE>(vn + v_off + c * (kBlk * 32));
                 }
 #pragma unroll
                 for (int t = 0; t < T; ++t) {
@@ -1020,7 +1027,10 @@ template <int D, int T, bool MASK>
 void launch_few(const Kv8AttnArgs& a, hipStream_t stream) {
     constexpr size_t lds = (size_t)kWaves * (16 * D + 64) * sizeof(float);
     static_assert(lds >= (size_t)T * (D / 32) * 2 * 64 * 16, "the queries lie where the results are joined");
-    hipLaunchKernelGGL((kv8_attn_few_kernel<D, T, MASK>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
+    if (a.once)
+        hipLaunchKernelGGL((kv8_attn_few_kernel<D, T, MASK, true>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
+    else
+        hipLaunchKernelGGL((kv8_attn_few_kernel<D, T, MASK, false>), dim3((unsigned)a.grid), dim3(kWaves * 64), lds, stream, a);
 }
 template <int D, bool MASK>
 void launch_pieces(const Kv8AttnArgs& a, hipStream_t stream) {
@@ -1057,6 +1067,11 @@ size_t kv8_attn_plan(Kv8AttnArgs& a) {
     const bool two = t32 == 2 && a.D == 128 && a.mode != SIXI_MASK_EXPLICIT;
     a.waves = t32 == 1 ? 1 : two ? 2 : kWaves;
     a.target = 2 * device_cu_count();  // (two work-groups on a CU)
+    // Codes that the 256 MB behind the L2 cannot hold until the next call go past it, where one work-group reads each
+    // (a token of 32 streams, 269 MB: 53 against 61 us; 8 streams of 256 dims, 320 MB: 66 against 73).  Fewer may
+    // still be there (one stream of 50k cells, 102 MB, called in turn with another: 38 against 35 the other way), and
+    // where several tiles read them, or the rows kernels, they are better kept (96 rows: 104 against 99).
+    a.once = a.code_bytes >= (int64_t)256 << 20;
     a.least = 4;
     const int64_t tiles = (t32 + a.waves - 1) / a.waves * a.Hkv * a.S;
     const int64_t blocks = (a.n_kv + kBlk - 1) / kBlk;

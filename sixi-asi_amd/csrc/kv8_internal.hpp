@@ -73,6 +73,8 @@ struct Kv8AttnArgs {
     int32_t least;                // blocks of a piece at least
     int32_t grid;                 // pieces at most
     int32_t cut;                  // whether cells may be cut (partial results in the workspace)
+    int64_t code_bytes;           // codes of all cells that a call may see
+    int32_t once;                 // codes are read past the caches
 };
 
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a, hipStream_t stream);

@@ -5,6 +5,7 @@
 // include/sixi_asi/common.hpp:40-67, negated).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 
@@ -231,6 +232,8 @@ int resolve_attn(const sixi_kv8_attn_params* p, sixi::Kv8AttnArgs* out, size_t* 
     a.scale_log2 = std::fmax(std::fabs(p->scale) * 1.4426950408889634f, 0x1p-85f);
     a.q_sign = std::signbit(p->scale) ? -1.0f : 1.0f;
     if ((a.n_q * (int64_t)a.G + 31) / 32 * a.Hkv * S > ((int64_t)1 << 23)) return SIXI_E_UNSUPPORTED;  // work-groups
+    // (pages that streams share are there once)
+    a.code_bytes = (paged ? std::min(S * blocks, c.n * sixi::kPageBlocks) : S * blocks) * sixi::kBlk * D * 2 * c.n_heads;
     a.part = static_cast<float*>(p->workspace);
     *ws = sixi::kv8_attn_plan(a);
     *out = a;

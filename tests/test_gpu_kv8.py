@@ -272,6 +272,31 @@ def test_attention_of_many_streams(s):
     _attend(s, 2, 2, 1, 128, cached, rows, 3104, seed=1)
 
 
+@pytest.mark.parametrize("d,n_q,H,masked", [(128, 1, 6, False), (128, 8, 6, False), (128, 5, 6, True), (256, 5, 6, False), (256, 3, 6, True),
+                                            (128, 40, 6, False)])
+def test_attention_in_a_cache_of_gigabytes(d, n_q, H, masked):
+    """A pool larger than the chip's caches, read past them where one work-group reads each cell: the same bits as a small
+    cache that holds the same cells."""
+    pages, n = (1 << 29) // (2 * PAGE * d) + 9, 2900
+    big, small = sa.Kv8Cache.empty(pages, PAGE, 1, d), sa.Kv8Cache.empty(1, 12 * PAGE, 1, d)
+    gen = torch.Generator(device="cuda").manual_seed(d + n_q)
+    table = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)[None].contiguous()
+    rows = [torch.randn((1, n + n_q, 1, d), generator=gen, device="cuda") for _ in range(2)]
+    sa.kv8_write(*rows, big, page_table=table)
+    sa.kv8_write(*rows, small)
+    q = torch.randn((1, n_q, H, d), generator=gen, device="cuda").half()
+    outs = [torch.zeros((1, n_q, H, d), device="cuda") for _ in range(2)]
+    mask = None
+    if masked:
+        mask = torch.full((1, 1, n_q, pages * PAGE), -float("inf"), dtype=torch.float16, device="cuda")
+        mask[..., :n] = torch.randn((n_q, n), generator=gen, device="cuda").half()
+    mode = sa.MASK_EXPLICIT if masked else sa.MASK_BLOCK_CAUSAL
+    for cache, out, pt in ((big, outs[0], table), (small, outs[1], None)):
+        m = None if mask is None else mask[..., :cache.n_blocks * BLOCK] if pt is None else mask
+        sa.Kv8Attention()(q, cache, out, kv_len=_i32([n]), q_len=_i32([n_q]), mask_mode=mode, mask=m, page_table=pt)
+    assert torch.equal(*outs) and bool((outs[0].abs().sum(-1) > 0).all())
+
+
 @pytest.mark.parametrize("d,n_q", [(128, 2), (128, 40), (256, 40)])
 def test_offsets_past_32_bits(d, n_q):
     """Blocks half a GiB apart: a stream's cells lie up to 5 GiB behind one another."""
