@@ -18,10 +18,10 @@
 // lane (n, h) of the 32 x 32 result holds cells 16h .. 16h + 15 of the block in order, which is what the
 // lane needs as its half of the next product's right operand.  So P never leaves its lane.
 //
-// Two kernels.  Up to 32 rows a group (decode), or 64 of 128 dims: the four waves of a work-group take blocks
+// Two forms.  Up to 32 rows a group (decode), or 64 of 128 dims: the four waves of a work-group take blocks
 // in turn, straight from memory into registers, one block ahead; nothing is shared but the queries.
-// More rows: NW waves take 32 rows each of the same cells; a step's codes are converted once, by all of them,
-// into f16 operands in LDS (two buffers, the next step's codes on their way in registers).
+// More rows: four waves take 32 rows each of the same cells; a step's codes are converted once, by all of them,
+// into f16 operands in LDS, the next step's codes on their way in registers (a kernel for each head dim).
 //
 // Work-groups: every stream's cells are cut into pieces of c blocks, c from the lengths on the device, so
 // that streams of any lengths fill the chip; pieces of one (stream, head, tile) are joined by a second
@@ -1062,7 +1062,7 @@ hipError_t launch(const Kv8AttnArgs& a, hipStream_t stream) {
 size_t kv8_attn_plan(Kv8AttnArgs& a) {
     const int64_t t32 = ((int64_t)a.n_q * a.G + 31) / 32;
     // 33 to 64 rows of 128 dims: both tiles in every wave's registers, where two of the rows kernel's four waves
-    // would only convert (32 streams of 48 rows, up to 16k cells: 75 against 95 us).  Not with a mask: its values
+    // would only convert (32 streams of 48 rows, up to 16k cells: 70 against 95 us).  Not with a mask: its values
     // do not fit beside them (32 streams of 60 rows: 175 against 118 us).
     const bool two = t32 == 2 && a.D == 128 && a.mode != SIXI_MASK_EXPLICIT;
     a.waves = t32 == 1 ? 1 : two ? 2 : kWaves;
